@@ -25,7 +25,8 @@ LIB_NAME = "libnvfp4dg.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
 SOURCES = ["dual_gemm.cu"]
-DEPS = ["dual_gemm.cu", "schedule.h", "sm100_ptx.cuh"]
+DEPS = ["dual_gemm.cu", "host.h", "quant.cuh", "schedule.h",
+        "sm100_ptx.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [

@@ -1,0 +1,45 @@
+// host.h — host state of the library (dual_gemm.cu) that its other translation
+// units use: the thread's error message, the device's properties and error
+// word, and tensor-map encoding.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <string>
+
+namespace nvfp4dg {
+
+// Device error word bits (role whose bounded wait expired).
+constexpr unsigned kErrProducer = 1u << 0;
+constexpr unsigned kErrMma = 1u << 1;
+constexpr unsigned kErrEpilogue = 1u << 2;
+constexpr unsigned kErrDrain = 1u << 3;
+
+struct HostDevice {
+  int id;
+  int sms;
+  unsigned* err;  // the device's error word
+};
+
+// The current device (an sm_100 one, or a status is returned).
+int host_device(HostDevice* out);
+
+// Message of the calling thread's last failure; both failure forms return the
+// status to hand to the caller.
+void host_clear_error();
+int host_fail(int code, const std::string& msg);
+int host_cuda_fail(cudaError_t e, const char* what);
+
+// Byte view of `layers` matrices, `layer_bytes` apart, of `rows` rows of
+// `row_bytes` bytes, `pitch` apart; boxes of 128 bytes x `box_rows` rows with
+// the 128-byte swizzle.  2-D for one layer, else 3-D.  Needs host_device()
+// first.
+int host_byte_map(const void* ptr, long long rows, long long row_bytes,
+                  long long pitch, int box_rows, long long layers,
+                  long long layer_bytes, CUtensorMap* out);
+
+// NVFP4DG_FLAG_SYNC_CHECK: waits for `stream` and reads the error word.
+int host_sync_check(cudaStream_t stream);
+
+}  // namespace nvfp4dg
