@@ -268,6 +268,141 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
                                           void* stream);
 
 /*
+ * NVFP4 product with bias, activation and residual in its epilogue: the
+ * projections around the dual GEMM (an FFN's down projection, attention's
+ * input and output projections),
+ *
+ *   C[m, n] = act(alpha * sum_k A[m, k] B[n, k] + bias[n]) * row_scale[m]
+ *             + residual[m, n]
+ *
+ * summed, activated and scaled in fp32 and rounded once to C's type.  A
+ * [M, K/2], SFA, B [N, K/2] and SFB are laid out as for the dual GEMM (dense
+ * rows; blocked scales padded to 128 rows).  M >= 0, N % 8 == 0, K a positive
+ * multiple of 64.  C and residual are row-major with row pitches of `ldc` /
+ * `ldr` elements (>= N, multiples of 8); residual may be C itself.  bias, row_scale
+ * and residual may be NULL.  All pointers are device pointers; A, B, SFA,
+ * SFB, C and residual 16-byte aligned.  No workspace is used.  The reference
+ * has no such product: its one kernel ends with the gated activation
+ * (nvfp4_dual_gemm.cu:126-193).
+ */
+#define NVFP4DG_ACT_NONE 0
+#define NVFP4DG_ACT_RELU 1
+#define NVFP4DG_ACT_SILU 2      /* x / (1 + e^-x)                             */
+#define NVFP4DG_ACT_GELU_TANH 3 /* x/2 (1 + tanh(sqrt(2/pi)(x + 0.044715x^3))) */
+#define NVFP4DG_ACT_GELU 4      /* x/2 (1 + erf(x / sqrt 2))                  */
+
+/* flags of nvfp4_linear_args (0 = automatic), beside
+ * NVFP4DG_FLAG_SYNC_CHECK and NVFP4DG_FLAG_NO_PDL: the tokens a tile holds
+ * and how many CTAs share a tile's K range (bits 8-10: 1 + log2, 0 =
+ * automatic; not for grouped products). */
+#define NVFP4DG_LINEAR_TOKENS32 (1u << 0)
+#define NVFP4DG_LINEAR_TOKENS64 (1u << 1)
+#define NVFP4DG_LINEAR_TOKENS128 (1u << 2)
+#define NVFP4DG_LINEAR_SPLIT_MASK 0x700u
+#define NVFP4DG_LINEAR_SPLIT(log2) ((1u + (log2)) << 8)
+
+typedef struct {
+  const void* A;
+  const void* B;
+  const void* SFA;
+  const void* SFB;
+  void* C;
+  const void* bias;       /* [N], or [groups, N] */
+  const void* residual;   /* [M, N] of C's type */
+  const float* row_scale; /* [M] */
+  long long ldc, ldr;
+  int M, N, K;
+  int c_dtype;    /* NVFP4DG_DTYPE_F16 or _BF16 */
+  int bias_dtype; /* NVFP4DG_DTYPE_F32 or C's */
+  int activation; /* NVFP4DG_ACT_* */
+  float alpha;
+  unsigned flags;
+} nvfp4_linear_args;
+
+NVFP4DG_API int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream);
+
+/*
+ * The same for `groups` (1..256) products that share N and K but have their
+ * own rows, weights and bias: the experts of a mixture, in one launch.  Group
+ * g owns rows [row0, row0 + group_rows[g]) of A, SFA, C, residual and
+ * row_scale (M rows in all), and batch g of B, SFB (per-batch sizes as for
+ * one product) and bias.  First rows are multiples of 128: group_row0, or,
+ * when it is NULL, each group starts at the next multiple of 128 after the
+ * one before.  Groups may be empty; rows of no group are not written.
+ *   on_device == 0: group_rows and group_row0 are host arrays, read during
+ *     the call; wrong or overlapping ones are refused.
+ *   on_device != 0: both are device arrays, read by the kernel (a router's
+ *     counts without a copy to the host; a captured call reads them at each
+ *     replay).  A negative count is an empty group; a group whose first row
+ *     lies outside A or is no multiple of 128 is empty, and one that reaches
+ *     past row M is cut there.  Groups must not overlap.
+ */
+NVFP4DG_API int nvfp4_linear_run_grouped(const nvfp4_linear_args* args,
+                                         const int* group_rows,
+                                         const int* group_row0, int groups,
+                                         int on_device, void* stream);
+
+/* The schedule nvfp4_linear_run would use: tokens per tile, CTAs per tile
+ * and CTAs in all.  Any out pointer may be NULL.  Host-only. */
+NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, unsigned flags,
+                                  int num_sms, int* tokens_out,
+                                  int* split_out, int* grid_out);
+
+/*
+ * Norms between two blocks of a transformer, fused with the gate and scale
+ * of the residual stream, for each of `rows` rows of D elements:
+ *
+ *   u = post ? norm(y) * post_weight + post_bias : y
+ *   r = x + scale * gate * u                  (rounded to the stream's type)
+ *   z = norm(r) * weight + bias               (of the rounded r)
+ *
+ * norm is v / sqrt(mean(v^2) + eps) (NVFP4DG_NORM_RMS) or
+ * (v - mean(v)) / sqrt(var(v) + eps) (NVFP4DG_NORM_LAYER), in fp32.  A NULL
+ * weight is 1, a NULL bias 0, a NULL gate 1.  With y == NULL, r is x and R is
+ * not written.  gate is [gate_rows, D] of the stream's type, row i of it for
+ * the i-th of gate_rows equal runs of rows (1: one gate for all; rows: one
+ * for each).  The stream x, y, R, Z have one type (F32, F16 or BF16) and
+ * their own row pitches in elements (multiples of 8 and >= D; F32: of 4); R
+ * may be x or y.  Weights and biases are F32 or of the stream's type
+ * (w_dtype).  Outputs of z, either or none:
+ *   Z              in the stream's type;
+ *   codes and sf   NVFP4 for the next product: [rows, D/2] e2m1 codes and
+ *                  blocked scales (every byte written, padding rows zero),
+ *                  equal bit for bit to nvfp4_quantize_rows of Z.  D % 64 == 0.
+ * D % 8 == 0, D <= 32768.  All pointers 16-byte aligned.  The reference has
+ * no counterpart: its harness hands it quantised activations
+ * (submission.py:1154).
+ */
+#define NVFP4DG_NORM_RMS 0
+#define NVFP4DG_NORM_LAYER 1
+
+typedef struct {
+  const void* x;
+  const void* y;
+  const void* weight;
+  const void* bias;
+  const void* post_weight;
+  const void* post_bias;
+  const void* gate;
+  void* R;
+  void* Z;
+  void* codes;
+  void* sf;
+  long long ldx, ldy, ldr, ldz;
+  int rows, D, gate_rows;
+  int dtype;   /* NVFP4DG_DTYPE_* of x, y, gate, R, Z */
+  int w_dtype; /* NVFP4DG_DTYPE_F32 or dtype */
+  int kind;    /* NVFP4DG_NORM_* */
+  int post;    /* norm y first */
+  float scale;
+  float eps;
+  unsigned flags; /* NVFP4DG_FLAG_NO_PDL or 0 */
+} nvfp4_block_norm_args;
+
+NVFP4DG_API int nvfp4_block_norm_run(const nvfp4_block_norm_args* args,
+                                     void* stream);
+
+/*
  * Read and clear the device error word of `device` (synchronizes that
  * device).  *word_out = 0 when no kernel reported a timeout; otherwise bits
  * identify the role whose bounded wait expired.  Returns a status code.

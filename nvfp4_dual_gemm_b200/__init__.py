@@ -5,6 +5,8 @@ the in-tree CUDA library ``libnvfp4dg.so`` behind the C ABI declared in
 ``include/nvfp4_dual_gemm.h``.
 """
 from .api import (  # noqa: F401
+    block_norm,
+    block_norm_nvfp4,
     cuda_nvfp4_dual_gemm,
     custom_kernel,
     dual_gemm,
@@ -15,6 +17,9 @@ from .api import (  # noqa: F401
     group_offsets,
     grouped_workspace_size,
     host_staging_size,
+    linear,
+    linear_grouped,
+    linear_plan,
     plan,
     plan_work,
     quantize_nvfp4,

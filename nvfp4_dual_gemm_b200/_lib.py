@@ -44,6 +44,21 @@ DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_BF16 = 2
 
+# nvfp4_linear_args: activations and schedule flags.
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_GELU = range(5)
+LINEAR_TOKENS32 = 1 << 0
+LINEAR_TOKENS64 = 1 << 1
+LINEAR_TOKENS128 = 1 << 2
+
+
+def linear_split(ctas: int) -> int:
+    """Flag bits that make ``ctas`` (1, 2, 4 or 8) CTAs share a tile."""
+    return (1 + {1: 0, 2: 1, 4: 2, 8: 3}[ctas]) << 8
+
+
+# nvfp4_block_norm_args: norms.
+NORM_RMS, NORM_LAYER = range(2)
+
 # Most weight slabs nvfp4_dual_gemm_run_host uses.
 MAX_HOST_SLABS = 16
 
@@ -56,6 +71,33 @@ _i = ctypes.c_int
 _u = ctypes.c_uint
 _sz = ctypes.c_size_t
 _ip = ctypes.POINTER(ctypes.c_int)
+
+
+class LinearArgs(ctypes.Structure):
+    """nvfp4_linear_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("A", "B", "SFA", "SFB", "C", "bias", "residual",
+                 "row_scale")] + \
+               [("ldc", ctypes.c_longlong), ("ldr", ctypes.c_longlong)] + \
+               [(n, ctypes.c_int) for n in
+                ("M", "N", "K", "c_dtype", "bias_dtype", "activation")] + \
+               [("alpha", ctypes.c_float), ("flags", ctypes.c_uint)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """nvfp4_block_norm_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("x", "y", "weight", "bias", "post_weight", "post_bias",
+                 "gate", "R", "Z", "codes", "sf")] + \
+               [(n, ctypes.c_longlong) for n in ("ldx", "ldy", "ldr",
+                                                 "ldz")] + \
+               [(n, ctypes.c_int) for n in
+                ("rows", "D", "gate_rows", "dtype", "w_dtype", "kind",
+                 "post")] + \
+               [("scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("flags", ctypes.c_uint)]
+
+
 SIGNATURES = {
     "nvfp4_dual_gemm_run": (_i, [_vp] * 7 + [_i, _i, _i, _i, _u, _vp]),
     "nvfp4_dual_gemm_workspace_size": (_sz, [_i, _i, _i, _i, _u]),
@@ -68,6 +110,11 @@ SIGNATURES = {
     "nvfp4_dual_gemm_run_grouped": (_i, [_vp] * 7 + [_ip, _ip, _i, _i, _i,
                                                      _u, _vp, _sz, _vp]),
     "nvfp4_dual_gemm_grouped_workspace_size": (_sz, [_ip, _i, _i, _i, _u]),
+    "nvfp4_linear_run": (_i, [ctypes.POINTER(LinearArgs), _vp]),
+    "nvfp4_linear_run_grouped": (_i, [ctypes.POINTER(LinearArgs), _vp, _vp,
+                                      _i, _i, _vp]),
+    "nvfp4_linear_plan": (_i, [_i, _i, _i, _u, _i, _ip, _ip, _ip]),
+    "nvfp4_block_norm_run": (_i, [ctypes.POINTER(BlockNormArgs), _vp]),
     "nvfp4_quantize": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp]),
     "nvfp4_quantize_rows": (_i, [_vp, _i, _i, _i, ctypes.c_longlong, _vp, _vp,
                                  _vp, _vp]),

@@ -32,6 +32,11 @@ __all__ = [
     "cuda_nvfp4_dual_gemm",
     "dual_gemm",
     "dual_gemm_host",
+    "linear",
+    "linear_grouped",
+    "linear_plan",
+    "block_norm",
+    "block_norm_nvfp4",
     "host_staging_size",
     "quantize_nvfp4",
     "scales_to_blocked",
@@ -278,6 +283,107 @@ def dual_gemm_grouped(A, B1, B2, SFA, SFB1, SFB2, C, group_rows,
             0 if workspace is None else workspace.numel(), _stream(dev))
     _lib.check(rc, "nvfp4_dual_gemm_run_grouped")
     return C
+
+
+def linear(A, B, SFA, SFB, C=None, *, bias=None, activation=None,
+           residual=None, row_scale=None, alpha: float = 1.0, dtype=None,
+           flags: int = 0) -> torch.Tensor:
+    """The NVFP4 product of the projections around the dual GEMM,
+    ``C = act(alpha * A B^T + bias) * row_scale + residual``, on the current
+    stream; returns C.
+
+    A [M, K/2] and B [N, K/2] with their blocked scales are as for
+    :func:`dual_gemm` (any M, N % 8 == 0, K a positive multiple of 64).
+    ``activation`` is None, "relu", "silu", "gelu_tanh" or "gelu"; ``bias``
+    [N] is float32 or of C's type, ``row_scale`` [M] float32, ``residual``
+    [M, N] of C's type (it may be C itself).  Without ``C``, a contiguous
+    output of ``dtype`` (default: the residual's type, else float16) is
+    allocated.  C and residual may have strided rows (pitches of multiples
+    of 8 elements).  Sums and the epilogue are fp32, rounded once.  Uses no
+    workspace and can be captured into a CUDA graph; inference only
+    (``nvfp4_linear_run``).  For one token up to a few the CTAs of a cluster
+    share each tile's K range; the result does not depend on timing."""
+    return _lib.ext().linear(A, B, SFA, SFB, C, bias=bias,
+                             activation=activation, residual=residual,
+                             row_scale=row_scale, alpha=alpha, dtype=dtype,
+                             flags=flags)
+
+
+def linear_grouped(A, B, SFA, SFB, C, group_rows, group_row0=None, *,
+                   bias=None, activation=None, row_scale=None,
+                   alpha: float = 1.0, flags: int = 0) -> torch.Tensor:
+    """:func:`linear` for the experts of a mixture, in one launch: group g
+    computes rows [row0[g], row0[g] + group_rows[g]) of C from the same rows
+    of A / SFA and expert g's weights (batch g of B [N, K/2, G] and of SFB, G
+    blocked layouts one after another) and bias (row g of [G, N]).
+    ``row_scale`` [rows of A] holds the routing weights.
+
+    ``group_rows`` and ``group_row0`` are sequences of ints, or int32 CUDA
+    tensors, which the kernel reads itself: a router's counts need no copy to
+    the host, and a captured call reads them at each replay.  Without
+    ``group_row0`` each group starts at the next multiple of 128
+    (:func:`group_offsets`).  Up to 256 groups, any of them empty; rows of no
+    group are not written.  Counts on the host are checked; on the device, a
+    group that is out of place is empty and one that reaches past the rows of
+    A or C is cut there (``nvfp4_linear_run_grouped``)."""
+    return _lib.ext().linear_grouped(A, B, SFA, SFB, C, group_rows,
+                                     group_row0, bias=bias,
+                                     activation=activation,
+                                     row_scale=row_scale, alpha=alpha,
+                                     flags=flags)
+
+
+def linear_plan(M: int, N: int, K: int, flags: int = 0,
+                num_sms: int = 148) -> dict:
+    """The schedule :func:`linear` would use (host-only; needs no GPU)."""
+    lib = _lib.load()
+    tokens, split, grid = (ctypes.c_int() for _ in range(3))
+    rc = lib.nvfp4_linear_plan(M, N, K, flags, num_sms, ctypes.byref(tokens),
+                               ctypes.byref(split), ctypes.byref(grid))
+    _lib.check(rc, "nvfp4_linear_plan")
+    return {"tokens": tokens.value, "split": split.value, "grid": grid.value}
+
+
+def block_norm(x, y=None, *, weight=None, bias=None, post_weight=None,
+               post_bias=None, gate=None, scale: float = 1.0,
+               kind: str = "rms", eps: float = 1e-6, post: bool = False,
+               pre: bool = True, R=None, Z=None, flags: int = 0):
+    """The norms between two blocks, fused with the gate and scale of the
+    residual stream; returns (R, Z)::
+
+        u = norm(y) * post_weight + post_bias   if post, else y
+        R = x + scale * gate * u                rounded to x's type
+        Z = norm(R) * weight + bias             (None with pre=False)
+
+    ``x`` [..., D] is the stream and ``y`` the block's output (float32,
+    float16 or bfloat16); without ``y``, R is x and only Z is computed.
+    ``kind`` is "rms" or "layer"; ``post`` is implied by ``post_weight`` or
+    ``post_bias``.  Weights and biases [D] are float32 or of x's type (one
+    type for all).  ``gate`` [G, D] (or [D]) holds one gate for each of G
+    equal runs of rows: 1 for a channel gate, the batch for one a sample, the
+    rows for one a row.  ``R`` and ``Z`` are allocated when not given; R may
+    be x or y.  [rows, D] tensors may have strided rows (16-byte pitches).
+    D % 8 == 0 up to 32768.  Inference only (``nvfp4_block_norm_run``)."""
+    return _lib.ext().block_norm(x, y, weight=weight, bias=bias,
+                                 post_weight=post_weight,
+                                 post_bias=post_bias, gate=gate, scale=scale,
+                                 kind=kind, eps=eps, post=post, pre=pre, R=R,
+                                 Z=Z, flags=flags)
+
+
+def block_norm_nvfp4(x, y=None, *, weight=None, bias=None, post_weight=None,
+                     post_bias=None, gate=None, scale: float = 1.0,
+                     kind: str = "rms", eps: float = 1e-6,
+                     post: bool = False, R=None, flags: int = 0):
+    """:func:`block_norm` with Z in NVFP4, for the next product
+    (:func:`dual_gemm`, :func:`linear`): returns (R, codes [rows, D/2],
+    blocked scales), equal bit for bit to :func:`quantize_nvfp4` of
+    :func:`block_norm`'s Z, which is never written.  D % 64 == 0."""
+    return _lib.ext().block_norm_nvfp4(x, y, weight=weight, bias=bias,
+                                       post_weight=post_weight,
+                                       post_bias=post_bias, gate=gate,
+                                       scale=scale, kind=kind, eps=eps,
+                                       post=post, R=R, flags=flags)
 
 
 def host_staging_size(M: int, N: int, K: int) -> int:

@@ -24,8 +24,8 @@ INCLUDE = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libnvfp4dg.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
-SOURCES = ["dual_gemm.cu"]
-DEPS = ["dual_gemm.cu", "host.h", "quant.cuh", "schedule.h",
+SOURCES = ["dual_gemm.cu", "linear.cu", "norm.cu"]
+DEPS = ["dual_gemm.cu", "linear.cu", "norm.cu", "host.h", "quant.cuh", "schedule.h",
         "sm100_ptx.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

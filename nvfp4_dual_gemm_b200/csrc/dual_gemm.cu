@@ -3305,7 +3305,7 @@ int host_device(HostDevice* out) {
 int host_byte_map(const void* ptr, long long rows, long long row_bytes,
                   long long pitch, int box_rows, long long layers,
                   long long layer_bytes, CUtensorMap* out) {
-  const int rank = layers > 1 ? 3 : 2;
+  const int rank = layers > 0 ? 3 : 2;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes),
                               static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(layers)};

@@ -33,8 +33,8 @@ int host_cuda_fail(cudaError_t e, const char* what);
 
 // Byte view of `layers` matrices, `layer_bytes` apart, of `rows` rows of
 // `row_bytes` bytes, `pitch` apart; boxes of 128 bytes x `box_rows` rows with
-// the 128-byte swizzle.  2-D for one layer, else 3-D.  Needs host_device()
-// first.
+// the 128-byte swizzle.  3-D, or 2-D for `layers` = 0 (one matrix).  Needs
+// host_device() first.
 int host_byte_map(const void* ptr, long long rows, long long row_bytes,
                   long long pitch, int box_rows, long long layers,
                   long long layer_bytes, CUtensorMap* out);

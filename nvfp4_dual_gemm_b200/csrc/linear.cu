@@ -1,0 +1,978 @@
+// linear.cu — NVFP4 products with a fused epilogue, and the same products
+// grouped by expert:
+//
+//   C[m, n] = act(alpha * sum_k A[m, k] B[n, k] + bias[n]) * row_scale[m]
+//             + residual[m, n]
+//
+// A (activations, [M, K]) and B (weights, [N, K]) are NVFP4 with blocked
+// scales, as for the dual GEMM; C is fp16 or bf16.
+//
+// linear_kernel gives the 128 TMEM lanes to the weights' rows and the
+// accumulator's columns to the tokens (C^T = B A^T): with few tokens, which
+// is where the product is bound by reading B once, the column side shrinks
+// to 32 while every lane still works, and a stage of the operand ring is
+// nearly all weights.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <string>
+
+#include "host.h"
+#include "nvfp4_dual_gemm.h"
+#include "sm100_ptx.cuh"
+
+namespace nvfp4dg {
+namespace {
+
+constexpr int kFeat = 128;          // features (rows of B) per tile
+constexpr int kRowBytes = 128;      // a stage holds 256 fp4 of K per row
+constexpr int kAtomBytes = 512;     // scales of 128 rows x 64 K elements
+constexpr int kRunBytes = 4 * kAtomBytes;
+constexpr int kThreads = 352;
+constexpr int kEpiWarps = 4;
+constexpr int kProdWWarp = 4;       // copies weights and their scales
+constexpr int kProdXWarp = 5;       // copies tokens and their scales
+constexpr int kMmaWarp = 6;
+constexpr int kSfWarp0 = 7;         // four warps, one per TMEM sub-partition
+constexpr int kSfWarps = 4;
+constexpr int kTmemCols = 512;
+constexpr int kMaxStages = 8;
+constexpr int kSfCols = 32;         // TMEM columns of a stage's scales
+constexpr int kMaxSplit = 8;
+constexpr int kMaxGroups = 256;
+constexpr int kSmemBudget = 221 * 1024;  // dynamic; static holds the groups
+
+struct LinearParams {
+  int M, N, K;       // M: rows of A and C (of all groups)
+  int kblocks;       // ceil(K / 256)
+  int n_tiles;       // ceil(N / 128)
+  int m_tiles;       // ceil(M / TN) (one problem)
+  int split;         // CTAs of a cluster that share a tile's K range
+  int stages;
+  const uint8_t* sfa;
+  const uint8_t* sfb;
+  long long sfb_group;  // bytes from one group's weight scales to the next
+  void* C;
+  long long ldc;
+  const void* bias;
+  int bias_f32;
+  const void* residual;
+  long long ldr;
+  const float* row_scale;
+  float alpha;
+  int act;
+  unsigned* err;
+  // grouped products: row counts and first rows, from device memory where
+  // dev_rows is set (dev_row0 may be null: each group starts at the next
+  // multiple of 128), else from the arrays here
+  int groups;
+  const int* dev_rows;
+  const int* dev_row0;
+  int rows[kMaxGroups];
+  int row0[kMaxGroups];
+};
+
+// Grouped products: group g owns rows [row0, row0 + rows) of A and C and
+// tiles [tile0[g], tile0[g + 1]).
+struct GroupTable {
+  int tile0[kMaxGroups + 1];
+  int row0[kMaxGroups];
+  int rows[kMaxGroups];
+};
+
+struct Tile {
+  int g;       // group (batch of B)
+  int n0;      // first feature
+  int x0;      // first row of A / C
+  int rows;    // valid rows from x0 (may exceed the tile)
+};
+
+// Built by one warp at the kernel's start.  Counts and first rows may come
+// from the device, so nothing about them was checked on the host: a group
+// whose first row is no multiple of 128 or lies outside the matrix gets no
+// rows, and no group reaches past row M.
+__device__ __forceinline__ void build_groups(const LinearParams& p, int tn,
+                                             int lane, GroupTable& tab) {
+  long long row_end = 0;
+  int tile_end = 0;
+  for (int base = 0; base < p.groups; base += 32) {
+    const int g = base + lane;
+    const bool in = g < p.groups;
+    int n = 0;
+    if (in) n = max(0, p.dev_rows ? p.dev_rows[g] : p.rows[g]);
+    // inclusive sums over the warp
+    long long pad = (static_cast<long long>(n) + 127) / 128 * 128;
+    const long long own = pad;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, pad, d);
+      if (lane >= d) pad += o;
+    }
+    long long r0 = row_end + pad - own;
+    row_end += __shfl_sync(0xffffffffu, pad, 31);
+    if (in) {
+      if (p.dev_rows == nullptr)
+        r0 = p.row0[g];
+      else if (p.dev_row0 != nullptr)
+        r0 = p.dev_row0[g];
+    }
+    if (r0 < 0 || r0 >= p.M || (r0 & 127)) n = 0;
+    n = static_cast<int>(
+        min(static_cast<long long>(n), max(p.M - r0, 0ll)));
+    int tiles = (n + tn - 1) / tn * p.n_tiles;
+    const int mine = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, tiles, d);
+      if (lane >= d) tiles += o;
+    }
+    if (in) {
+      tab.tile0[g] = tile_end + tiles - mine;
+      tab.row0[g] = n ? static_cast<int>(r0) : 0;
+      tab.rows[g] = n;
+    }
+    tile_end += __shfl_sync(0xffffffffu, tiles, 31);
+  }
+  if (lane == 0) tab.tile0[p.groups] = tile_end;
+}
+
+// Token tiles fastest, so that CTAs of neighbouring tiles read the same
+// weights at the same time.
+template <int TN>
+__device__ __forceinline__ Tile locate(const LinearParams& p,
+                                       const GroupTable& tab, int tile) {
+  Tile t;
+  if (p.groups == 0) {
+    const int nt = tile / p.m_tiles;
+    t.g = 0;
+    t.n0 = nt * kFeat;
+    t.x0 = (tile - nt * p.m_tiles) * TN;
+    t.rows = p.M - t.x0;
+    return t;
+  }
+  // the last group whose first tile is <= tile (empty groups have none)
+  int lo = 0, hi = p.groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.tile0[mid] <= tile)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int local = tile - tab.tile0[lo];
+  const int mt = (tab.rows[lo] + TN - 1) / TN;
+  const int nt = local / mt;
+  const int m0 = (local - nt * mt) * TN;
+  t.g = lo;
+  t.n0 = nt * kFeat;
+  t.x0 = tab.row0[lo] + m0;
+  t.rows = tab.rows[lo] - m0;
+  return t;
+}
+
+// 4 consecutive 32-bit TMEM columns of this warp's 32 lanes.
+__device__ __forceinline__ void tc_ld_4cols(uint32_t taddr, float (&v)[4]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+  return __half2float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// act(v), NC values, in fp32.  silu(x) = x / (1 + e^-x);
+// 0.5 (1 + tanh u) = 1 / (1 + e^-2u), so the tanh form of gelu is
+// x / (1 + e^-2u) with u = sqrt(2/pi) (x + 0.044715 x^3); the erf form is
+// 0.5 x erfc(-x / sqrt 2), which keeps its digits for negative x.
+template <int NC>
+__device__ __forceinline__ void activate(float (&v)[NC], int act) {
+  if (act == NVFP4DG_ACT_NONE) return;
+  if (act == NVFP4DG_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // keeps NaN
+  } else if (act == NVFP4DG_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
+  } else if (act == NVFP4DG_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const float x = v[i];
+      const float m2u = -1.5957691216057308f * x * fmaf(0.044715f, x * x, 1.f);
+      v[i] = __fdividef(x, 1.f + __expf(m2u));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      v[i] = 0.5f * v[i] * erfcf(-0.7071067811865476f * v[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float load_bias(const LinearParams& p, int g,
+                                           int n) {
+  if (p.bias == nullptr || n >= p.N) return 0.f;
+  const size_t i = (size_t)g * p.N + n;
+  return p.bias_f32 ? static_cast<const float*>(p.bias)[i]
+                    : to_f32<T>(static_cast<const T*>(p.bias)[i]);
+}
+
+// Residual of NC rows of C from row x (valid: `nv` of them), feature n.
+template <typename T, int NC>
+__device__ __forceinline__ void load_residual(const LinearParams& p, int x,
+                                              int n, int nv, T (&r)[NC]) {
+  if (p.residual == nullptr) return;
+  const T* src = static_cast<const T*>(p.residual) + (size_t)x * p.ldr + n;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (i < nv) r[i] = src[(size_t)i * p.ldr];
+}
+
+// Epilogue of NC rows (tokens) of one feature: the accumulators v to C.
+template <typename T, int NC>
+__device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
+                                       int nv, float bias, const T (&r)[NC],
+                                       float (&v)[NC]) {
+#pragma unroll
+  for (int i = 0; i < NC; ++i) v[i] = fmaf(p.alpha, v[i], bias);
+  activate<NC>(v, p.act);
+  if (p.row_scale != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (i < nv) v[i] *= p.row_scale[x + i];
+  }
+  if (p.residual != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) v[i] += to_f32<T>(r[i]);
+  }
+  T* dst = static_cast<T*>(p.C) + (size_t)x * p.ldc + n;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (i < nv) dst[(size_t)i * p.ldc] = from_f32<T>(v[i]);
+}
+
+template <int TN>
+struct Cfg {
+  static constexpr int kWBytes = kFeat * kRowBytes;
+  static constexpr int kXBytes = TN * kRowBytes;
+  static constexpr int kStageBytes = kWBytes + kXBytes + 2 * kRunBytes;
+  // split-K: the partials a CTA receives, fp32
+  static constexpr int kRecvBytes = kFeat * TN * 4;
+  static constexpr int kSfBase = 2 * TN;  // two accumulators, then scales
+  static constexpr int kTmemStages = (kTmemCols - kSfBase) / kSfCols;
+  static constexpr int stages(int split) {
+    const int room = kSmemBudget - 1024 - (split > 1 ? kRecvBytes : 0);
+    const int s = room / kStageBytes;
+    const int cap = kTmemStages < kMaxStages ? kTmemStages : kMaxStages;
+    return s < cap ? s : cap;
+  }
+  static constexpr int smem(int split) {
+    return stages(split) * kStageBytes + (split > 1 ? kRecvBytes : 0) + 1024;
+  }
+  static_assert(kStageBytes % 1024 == 0, "stages stay 1024-byte aligned");
+};
+
+// Per 256-wide K block the two producer warps copy a [128 x 128 B] weight
+// tile, a [TN x 128 B] token tile and their scale runs into a ring stage;
+// four scale warps move the scales into TMEM; one thread issues four
+// block-scaled MMAs (M = 128 features, N = TN tokens, K = 64) and four warps
+// finish the tile.  Two accumulators, so that a tile's epilogue runs under
+// the next tile's products.  K needs only be a multiple of 64: the last
+// block's missing 64-wide steps are not issued.
+//
+// split > 1: the CTAs of a cluster share one tile's K range.  Each sends the
+// fp32 partials of the other ranks' token columns into their shared memory
+// and finishes its own share, adding the partials in rank order.
+template <typename T, int TN>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap tmW,
+                  const __grid_constant__ CUtensorMap tmX,
+                  const __grid_constant__ LinearParams p) {
+  using Cf = Cfg<TN>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t sfdata_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t empty_bar[kMaxStages];
+  __shared__ __align__(8) uint64_t acc_full_bar[2];
+  __shared__ __align__(8) uint64_t acc_empty_bar[2];
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ __align__(8) uint64_t recv_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ GroupTable tab;
+
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const int S = p.stages;
+  const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+
+  if (warp == 0) {
+    uint64_t* bar = nullptr;
+    uint32_t count = 1;
+    if (lane < 8) {
+      bar = full_bar + lane;
+      count = 2 + kSfWarps;  // both producers and the scale warps
+    } else if (lane < 16) {
+      bar = sfdata_bar + (lane - 8);
+      count = 2;
+    } else if (lane < 24) {
+      bar = empty_bar + (lane - 16);
+    } else if (lane < 26) {
+      bar = acc_full_bar + (lane - 24);
+    } else if (lane < 28) {
+      bar = acc_empty_bar + (lane - 26);
+      count = kEpiWarps;
+    } else if (lane == 28) {
+      bar = &drain_bar;
+    } else if (lane == 29) {
+      bar = &recv_bar;
+    }
+    if (bar != nullptr) {
+      mbar_init(bar, count);
+      fence_mbar_init();
+    }
+    if (lane == 30) prefetch_tmap(&tmW);
+    if (lane == 31) prefetch_tmap(&tmX);
+    if (lane == 0) s_wait_failed = 0u;
+    fence_proxy_async_smem();
+    __syncwarp();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&tmem_base_sh, kTmemCols);
+    tmem_relinquish();
+  }
+  // the barriers of every CTA of the cluster before any remote use
+  if (p.split > 1) cluster_arrive_relaxed();
+  griddep_launch_dependents();
+  if (p.groups > 0 && warp == 1) {
+    if (p.dev_rows != nullptr) griddep_wait();
+    build_groups(p, TN, lane, tab);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (p.split > 1) cluster_wait();
+  const uint32_t tmem = tmem_base_sh;
+
+  const int total =
+      p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
+  const int first = static_cast<int>(blockIdx.x) / p.split;
+  const int step = static_cast<int>(gridDim.x) / p.split;
+  const int kb0 = static_cast<int>((long long)p.kblocks * rank / p.split);
+  const int kb1 =
+      static_cast<int>((long long)p.kblocks * (rank + 1) / p.split);
+  const int kblk64 = p.K / 64;
+
+  if (warp == kProdWWarp || warp == kProdXWarp) {
+    // ---------------------------------------------------------- producers
+    if (lane == 0) {
+      const bool w_side = warp == kProdWWarp;
+      const CUtensorMap* tm = w_side ? &tmW : &tmX;
+      const uint64_t pol = w_side ? kPolicyEvictNormal : kPolicyEvictLast;
+      const uint32_t tile_bytes = w_side ? Cf::kWBytes : Cf::kXBytes;
+      const uint32_t tile_off = w_side ? 0 : Cf::kWBytes;
+      const uint32_t sf_off =
+          Cf::kWBytes + Cf::kXBytes + (w_side ? 0 : kRunBytes);
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      griddep_wait();  // global memory only after the previous grid
+      for (int tile = first; ok && tile < total; tile += step) {
+        const Tile t = locate<TN>(p, tab, tile);
+        const uint8_t* sf =
+            w_side ? p.sfb + (size_t)t.g * p.sfb_group +
+                         (size_t)(t.n0 / 128) * kblk64 * kAtomBytes
+                   : p.sfa + (size_t)(t.x0 / 128) * kblk64 * kAtomBytes;
+        const int row = w_side ? t.n0 : t.x0;
+        const int layer = w_side ? t.g : 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (issued >= S &&
+              !mbar_wait(&empty_bar[stage], phase ^ 1u, p.err,
+                         kErrProducer)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + stage * Cf::kStageBytes;
+          const uint32_t run =
+              static_cast<uint32_t>(min(4, kblk64 - 4 * kb)) * kAtomBytes;
+          mbar_arrive_expect_tx(&sfdata_bar[stage], run);
+          bulk_load(st + sf_off, sf + (size_t)kb * kRunBytes, run,
+                    &sfdata_bar[stage], pol);
+          mbar_arrive_expect_tx(&full_bar[stage], tile_bytes);
+          tma_load_3d(st + tile_off, tm, &full_bar[stage], kb * kRowBytes,
+                      row, layer, pol);
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // never leave with copies in flight
+      for (int s = 0; s < S; ++s) {
+        if (issued > s) {
+          const uint32_t par =
+              static_cast<uint32_t>(((issued - 1 - s) / S) & 1);
+          mbar_wait(&sfdata_bar[s], par, p.err, kErrDrain, false);
+          mbar_wait(&full_bar[s], par, p.err, kErrDrain, false);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kSfWarp0) {
+    // ---------------------------------------------------------- scale warps
+    // Lane 32q + i, column c of a K step's four columns holds the scales of
+    // rows i + 32c of the 128-row block.  A tile of TN < 128 tokens starts
+    // at column (x0 % 128) / 32 of its block.
+    const uint32_t q = static_cast<uint32_t>(warp % 4);
+    const uint32_t t_lane = tmem + ((32u * q) << 16);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    griddep_wait();
+    for (int tile = first; ok && tile < total; tile += step) {
+      const int part =
+          TN == 128 ? 0 : (locate<TN>(p, tab, tile).x0 % 128) / 32;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        const bool got = mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        const uint32_t sf_s = smem_u32(smem + stage * Cf::kStageBytes +
+                                       Cf::kWBytes + Cf::kXBytes) +
+                              16u * lane;
+        uint32_t r[32];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 w = lds128(sf_s + j * kAtomBytes);
+          const uint4 x = lds128(sf_s + kRunBytes + j * kAtomBytes);
+          r[4 * j + 0] = w.x;
+          r[4 * j + 1] = w.y;
+          r[4 * j + 2] = w.z;
+          r[4 * j + 3] = w.w;
+          if (TN == 128) {
+            r[16 + 4 * j + 0] = x.x;
+            r[16 + 4 * j + 1] = x.y;
+          } else if (TN == 64) {
+            r[16 + 4 * j + 0] = part ? x.z : x.x;
+            r[16 + 4 * j + 1] = part ? x.w : x.y;
+          } else {
+            r[16 + 4 * j + 0] =
+                part < 2 ? (part ? x.y : x.x) : (part == 2 ? x.z : x.w);
+            r[16 + 4 * j + 1] = x.y;
+          }
+          r[16 + 4 * j + 2] = x.z;
+          r[16 + 4 * j + 3] = x.w;
+        }
+        __syncwarp();
+        tc_st_32cols(t_lane + Cf::kSfBase + stage * kSfCols, r);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_bar[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = idesc_nvf4(kFeat, TN);
+      const uint64_t w_desc0 =
+          smem_desc(smem_u32(smem), 16, 1024, SmemLayout::kSwizzle128B);
+      const uint64_t x_desc0 = smem_desc(smem_u32(smem) + Cf::kWBytes, 16,
+                                         1024, SmemLayout::kSwizzle128B);
+      int stage = 0;
+      uint32_t phase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += step, ++it) {
+        const int a = it & 1;
+        if (!mbar_wait(&acc_empty_bar[a], ((it >> 1) & 1) ^ 1u, p.err,
+                       kErrMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d = tmem + a * TN;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, p.err, kErrMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t soff =
+              static_cast<uint32_t>(stage) * (Cf::kStageBytes >> 4);
+          const uint32_t sf_t = tmem + Cf::kSfBase + stage * kSfCols;
+          const int steps = min(4, kblk64 - 4 * kb);
+          for (int j = 0; j < steps; ++j)
+            tc_mma_nvf4(d, w_desc0 + soff + 2u * j, x_desc0 + soff + 2u * j,
+                        kIdesc, sf_t + 4 * j, sf_t + 16 + 4 * j,
+                        (kb > kb0 || j > 0) ? 1u : 0u);
+          tc_commit(&empty_bar[stage]);
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) tc_commit(&acc_full_bar[a]);
+      }
+      // no MMA may still be running when TMEM is released
+      tc_commit(&drain_bar);
+      mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
+    }
+    __syncwarp();
+  } else if (p.split == 1) {
+    // ---------------------------------------------------------- epilogue
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    int it = 0;
+    griddep_wait();
+    for (int tile = first; tile < total; tile += step, ++it) {
+      const Tile t = locate<TN>(p, tab, tile);
+      const int a = it & 1;
+      const int n = t.n0 + threadIdx.x;
+      const float bias = load_bias<T>(p, t.g, n);
+      const int rows = n < p.N ? min(t.rows, TN) : 0;
+      const bool got =
+          mbar_wait(&acc_full_bar[a], (it >> 1) & 1, p.err, kErrEpilogue);
+      if (!__all_sync(0xffffffffu, got)) break;
+      tc_fence_after();
+      const int last = (min(t.rows, TN) - 1) / 32;
+#pragma unroll 1
+      for (int c = 0; c <= last; ++c) {
+        T r[32];
+        float v[32];
+        load_residual<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, r);
+        __syncwarp();
+        tc_ld_32cols(t_row + a * TN + 32 * c, v);
+        tc_wait_ld();
+        tie32(v);
+        if (c == last) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc_empty_bar[a]);
+        }
+        finish<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, bias, r, v);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- split-K
+    // Groups of four token columns; rank d finishes groups
+    // [d * gpr, (d + 1) * gpr).  In the receive buffer, source s, own group
+    // j, row r sit at ((s * gpr + j) * 128 + r) * 16.
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int row = threadIdx.x;
+    const Tile t = locate<TN>(p, tab, first);
+    const int nv = min(t.rows, TN);
+    const int g4 = (nv + 3) / 4;
+    const int gpr = (g4 + p.split - 1) / p.split;
+    const int g_own = rank * gpr;
+    const int n_own = max(0, min(gpr, g4 - g_own));
+    const uint32_t recv = smem_u32(smem + S * Cf::kStageBytes);
+    if (threadIdx.x == 0 && n_own > 0)
+      mbar_arrive_expect_tx(&recv_bar, (p.split - 1) * n_own * 2048);
+    griddep_wait();
+    const int n = t.n0 + row;
+    const float bias = load_bias<T>(p, t.g, n);
+    const bool got = mbar_wait(&acc_full_bar[0], 0, p.err, kErrEpilogue);
+    if (__all_sync(0xffffffffu, got)) {
+      tc_fence_after();
+      int d = 0, j = 0;  // rank and its group
+      uint32_t dst = 0, bar = 0;
+#pragma unroll 1
+      for (int c = 0; 8 * c < g4; ++c) {
+        float v[32];
+        __syncwarp();
+        tc_ld_32cols(t_row + 32 * c, v);
+        tc_wait_ld();
+        tie32(v);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (8 * c + q < g4) {
+            if (j == 0) {
+              dst = mapa_shared(recv, d);
+              bar = mapa_shared(smem_u32(&recv_bar), d);
+            }
+            if (d != rank) {
+              const float f[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2],
+                                  v[4 * q + 3]};
+              st_async_v4(dst + ((rank * gpr + j) * 128u + row) * 16u, f,
+                          bar);
+            }
+            if (++j == gpr) {
+              j = 0;
+              ++d;
+            }
+          }
+        }
+      }
+      bool landed = false;
+#pragma unroll 1
+      for (int o = 0; o < n_own; ++o) {
+        const int col = 4 * (g_own + o);
+        const int rows = n < p.N ? nv - col : 0;
+        T r[4];
+        float own[4], v[4] = {0.f, 0.f, 0.f, 0.f};
+        load_residual<T, 4>(p, t.x0 + col, n, rows, r);
+        __syncwarp();
+        tc_ld_4cols(t_row + col, own);
+        tc_wait_ld();
+        if (!landed) {
+          const bool in = mbar_wait(&recv_bar, 0, p.err, kErrEpilogue);
+          if (!__all_sync(0xffffffffu, in)) break;
+          landed = true;
+        }
+        for (int s = 0; s < p.split; ++s) {
+          if (s == rank) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += own[i];
+          } else {
+            const uint4 u = lds128(recv + ((s * gpr + o) * 128u + row) * 16u);
+            v[0] += __uint_as_float(u.x);
+            v[1] += __uint_as_float(u.y);
+            v[2] += __uint_as_float(u.z);
+            v[3] += __uint_as_float(u.w);
+          }
+        }
+        finish<T, 4>(p, t.x0 + col, n, rows, bias, r, v);
+      }
+    }
+  }
+
+  // ------------------------------------------------------------ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (p.split > 1) cluster_sync_final();
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+struct LinearPlan {
+  int tn;      // tokens per tile
+  int split;   // CTAs that share a tile's K range
+  int grid;    // CTAs
+  int tiles;
+};
+
+LinearPlan plan_linear(long long m_tiles32, long long m_tiles64,
+                       long long m_tiles128, int N, int K, int groups,
+                       unsigned flags, int sms) {
+  LinearPlan pl{};
+  const int n_tiles = (N + kFeat - 1) / kFeat;
+  const int kblocks = (K + 255) / 256;
+  // the narrowest tile that holds as few tiles as the widest: columns beyond
+  // the tokens cost shared memory and MMA time
+  if (flags & NVFP4DG_LINEAR_TOKENS32)
+    pl.tn = 32;
+  else if (flags & NVFP4DG_LINEAR_TOKENS64)
+    pl.tn = 64;
+  else if (flags & NVFP4DG_LINEAR_TOKENS128)
+    pl.tn = 128;
+  else
+    pl.tn = m_tiles32 == m_tiles128 ? 32 : m_tiles64 == m_tiles128 ? 64 : 128;
+  const long long mt =
+      pl.tn == 32 ? m_tiles32 : pl.tn == 64 ? m_tiles64 : m_tiles128;
+  pl.tiles = static_cast<int>(std::min<long long>(mt * n_tiles, 1 << 30));
+  pl.split = 1;
+  const int forced =
+      static_cast<int>((flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8);
+  if (groups == 0 && forced > 0) {
+    pl.split = 1 << (forced - 1);
+  } else if (groups == 0) {
+    for (int s = kMaxSplit; s > 1; s /= 2)
+      if ((long long)pl.tiles * s <= sms && kblocks >= 2 * s) {
+        pl.split = s;
+        break;
+      }
+  }
+  pl.split = std::min(pl.split, std::max(kblocks, 1));
+  while (pl.split & (pl.split - 1)) --pl.split;
+  pl.grid = pl.split > 1 ? pl.tiles * pl.split : std::min(pl.tiles, sms);
+  return pl;
+}
+
+template <typename T, int TN>
+int launch_linear(const LinearParams& kp, const LinearPlan& pl,
+                  const CUtensorMap& tw, const CUtensorMap& tx, int dev,
+                  unsigned flags, cudaStream_t stream) {
+  static std::atomic<unsigned long long> ready{0};
+  auto kernel = linear_kernel<T, TN>;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(ready.load() & bit)) {
+    const int most = std::max(Cfg<TN>::smem(1), Cfg<TN>::smem(2));
+    cudaError_t e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
+    ready.fetch_or(bit);
+  }
+  LinearParams p = kp;
+  p.stages = Cfg<TN>::stages(pl.split);
+  p.m_tiles = (p.M + TN - 1) / TN;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg<TN>::smem(pl.split);
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  unsigned na = 0;
+  if (!(flags & NVFP4DG_FLAG_NO_PDL)) {
+    attrs[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[na].val.programmaticStreamSerializationAllowed = 1;
+    ++na;
+  }
+  if (pl.split > 1) {
+    attrs[na].id = cudaLaunchAttributeClusterDimension;
+    attrs[na].val.clusterDim.x = pl.split;
+    attrs[na].val.clusterDim.y = 1;
+    attrs[na].val.clusterDim.z = 1;
+    ++na;
+  }
+  cfg.attrs = attrs;
+  cfg.numAttrs = na;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tw, tx, p);
+  if (e != cudaSuccess) return host_cuda_fail(e, "linear_kernel launch");
+  return NVFP4DG_OK;
+}
+
+int check_linear(const nvfp4_linear_args* a, int groups,
+                 bool placed_on_device) {
+  if (a == nullptr) return host_fail(NVFP4DG_ERR_INVALID, "args is NULL");
+  if (a->M < 0 || a->N < 0 || a->K < 0)
+    return host_fail(NVFP4DG_ERR_INVALID, "M, N, K must be non-negative");
+  if (a->N % 8 != 0)
+    return host_fail(NVFP4DG_ERR_INVALID, "N must be a multiple of 8");
+  if (a->K == 0 || a->K % 64 != 0)
+    return host_fail(NVFP4DG_ERR_INVALID,
+                     "K must be a positive multiple of 64");
+  if (a->c_dtype != NVFP4DG_DTYPE_F16 && a->c_dtype != NVFP4DG_DTYPE_BF16)
+    return host_fail(NVFP4DG_ERR_INVALID, "C must be F16 or BF16");
+  if (a->bias != nullptr && a->bias_dtype != NVFP4DG_DTYPE_F32 &&
+      a->bias_dtype != a->c_dtype)
+    return host_fail(NVFP4DG_ERR_INVALID, "bias must be F32 or of C's type");
+  if (a->activation < NVFP4DG_ACT_NONE || a->activation > NVFP4DG_ACT_GELU)
+    return host_fail(NVFP4DG_ERR_INVALID, "unknown activation");
+  const unsigned t = a->flags & (NVFP4DG_LINEAR_TOKENS32 |
+                                 NVFP4DG_LINEAR_TOKENS64 |
+                                 NVFP4DG_LINEAR_TOKENS128);
+  if (t & (t - 1))
+    return host_fail(NVFP4DG_ERR_INVALID, "the TOKENS flags are exclusive");
+  const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
+                         NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_SPLIT_MASK |
+                         NVFP4DG_FLAG_SYNC_CHECK | NVFP4DG_FLAG_NO_PDL;
+  if (a->flags & ~known)
+    return host_fail(NVFP4DG_ERR_INVALID, "unknown flag bits");
+  if (((a->flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8) > 4)
+    return host_fail(NVFP4DG_ERR_INVALID, "split must be 1, 2, 4 or 8");
+  if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
+  // tile numbers are 32-bit; groups placed by the device may overlap, so each
+  // of them counts as all rows
+  const long long per = groups && placed_on_device ? groups : 1;
+  if (((a->M + 31ll) / 32 * per + groups) * ((a->N + 127ll) / 128) >=
+          (1ll << 30) ||
+      a->M > (1 << 30) || a->N > (1 << 30) || a->K > (1 << 30))
+    return host_fail(NVFP4DG_ERR_INVALID, "too many tiles (M * N too large)");
+  if (a->C == nullptr) return host_fail(NVFP4DG_ERR_INVALID, "C is NULL");
+  if (a->ldc < a->N || (a->residual != nullptr && a->ldr < a->N))
+    return host_fail(NVFP4DG_ERR_INVALID,
+                     "the row pitch of C and residual must be at least N");
+  const void* ops[4] = {a->A, a->B, a->SFA, a->SFB};
+  const char* names[4] = {"A", "B", "SFA", "SFB"};
+  for (int i = 0; i < 4; ++i) {
+    if (ops[i] == nullptr)
+      return host_fail(NVFP4DG_ERR_INVALID,
+                       std::string(names[i]) + " is NULL");
+    if (reinterpret_cast<uintptr_t>(ops[i]) % 16 != 0)
+      return host_fail(NVFP4DG_ERR_ALIGN, std::string(names[i]) +
+                                              " is not 16-byte aligned");
+  }
+  if (reinterpret_cast<uintptr_t>(a->C) % 16 || a->ldc % 8 ||
+      reinterpret_cast<uintptr_t>(a->residual) % 16 ||
+      (a->residual != nullptr && a->ldr % 8))
+    return host_fail(NVFP4DG_ERR_ALIGN,
+                     "C, residual and their row pitches must be 16-byte "
+                     "aligned");
+  const size_t be = a->bias_dtype == NVFP4DG_DTYPE_F32 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(a->bias) % be ||
+      reinterpret_cast<uintptr_t>(a->row_scale) % 4)
+    return host_fail(NVFP4DG_ERR_ALIGN,
+                     "bias and row_scale must be aligned to their elements");
+  return NVFP4DG_OK;
+}
+
+int run_linear(const nvfp4_linear_args* a, const int* group_rows,
+               const int* group_row0, int groups, bool on_device,
+               void* stream_ptr) {
+  host_clear_error();
+  int rc = check_linear(a, groups, on_device && group_row0 != nullptr);
+  if (rc) return rc;
+  if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
+  LinearParams p;
+  std::memset(&p, 0, sizeof(p));
+  long long mt[3] = {0, 0, 0};
+  if (groups > 0 && !on_device) {
+    long long next = 0;
+    for (int g = 0; g < groups; ++g) {
+      const long long n = group_rows[g];
+      const long long r0 = group_row0 ? group_row0[g] : next;
+      if (n < 0 || r0 < 0 || r0 % 128 != 0)
+        return host_fail(NVFP4DG_ERR_INVALID,
+                         "group " + std::to_string(g) +
+                             ": rows must be >= 0 and the first row a "
+                             "multiple of 128");
+      if (n > 0 && r0 < next)
+        return host_fail(NVFP4DG_ERR_INVALID,
+                         "group " + std::to_string(g) +
+                             " overlaps the previous one (each group's rows "
+                             "are rounded up to 128)");
+      if (n > 0 && r0 + n > a->M)
+        return host_fail(NVFP4DG_ERR_INVALID,
+                         "group " + std::to_string(g) +
+                             " reaches past the " + std::to_string(a->M) +
+                             " rows of A");
+      if (n > 0) next = r0 + (n + 127) / 128 * 128;
+      p.rows[g] = static_cast<int>(n);
+      p.row0[g] = n > 0 ? static_cast<int>(r0) : 0;
+      mt[0] += (n + 31) / 32;
+      mt[1] += (n + 63) / 64;
+      mt[2] += (n + 127) / 128;
+    }
+    if (mt[0] == 0) return NVFP4DG_OK;
+  } else {
+    // counts on the device: A's rows spread evenly
+    const long long per = groups ? (a->M + groups - 1) / groups : a->M;
+    const long long g = groups ? groups : 1;
+    mt[0] = (per + 31) / 32 * g;
+    mt[1] = (per + 63) / 64 * g;
+    mt[2] = (per + 127) / 128 * g;
+  }
+  HostDevice dev;
+  if ((rc = host_device(&dev))) return rc;
+  LinearPlan pl = plan_linear(mt[0], mt[1], mt[2], a->N, a->K, groups,
+                              a->flags, dev.sms);
+  if (groups > 0 && on_device) pl.grid = dev.sms;
+  p.M = a->M;
+  p.N = a->N;
+  p.K = a->K;
+  p.kblocks = (a->K + 255) / 256;
+  p.n_tiles = (a->N + kFeat - 1) / kFeat;
+  p.split = pl.split;
+  p.sfa = static_cast<const uint8_t*>(a->SFA);
+  p.sfb = static_cast<const uint8_t*>(a->SFB);
+  p.sfb_group = (a->N + 127ll) / 128 * (a->K / 64) * kAtomBytes;
+  p.C = a->C;
+  p.ldc = a->ldc;
+  p.bias = a->bias;
+  p.bias_f32 = a->bias_dtype == NVFP4DG_DTYPE_F32;
+  p.residual = a->residual;
+  p.ldr = a->ldr;
+  p.row_scale = a->row_scale;
+  p.alpha = a->alpha;
+  p.act = a->activation;
+  p.err = dev.err;
+  p.groups = groups;
+  p.dev_rows = on_device ? group_rows : nullptr;
+  p.dev_row0 = on_device ? group_row0 : nullptr;
+  CUtensorMap tw, tx;
+  const long long kb = a->K / 2;
+  if ((rc = host_byte_map(a->B, a->N, kb, kb, kFeat, std::max(groups, 1),
+                          a->N * kb, &tw)))
+    return rc;
+  if ((rc = host_byte_map(a->A, a->M, kb, kb, pl.tn, 1, a->M * kb, &tx)))
+    return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  const bool bf = a->c_dtype == NVFP4DG_DTYPE_BF16;
+  if (pl.tn == 32)
+    rc = bf ? launch_linear<__nv_bfloat16, 32>(p, pl, tw, tx, dev.id,
+                                               a->flags, stream)
+            : launch_linear<__half, 32>(p, pl, tw, tx, dev.id, a->flags,
+                                        stream);
+  else if (pl.tn == 64)
+    rc = bf ? launch_linear<__nv_bfloat16, 64>(p, pl, tw, tx, dev.id,
+                                               a->flags, stream)
+            : launch_linear<__half, 64>(p, pl, tw, tx, dev.id, a->flags,
+                                        stream);
+  else
+    rc = bf ? launch_linear<__nv_bfloat16, 128>(p, pl, tw, tx, dev.id,
+                                                a->flags, stream)
+            : launch_linear<__half, 128>(p, pl, tw, tx, dev.id, a->flags,
+                                         stream);
+  if (rc) return rc;
+  return (a->flags & NVFP4DG_FLAG_SYNC_CHECK) ? host_sync_check(stream)
+                                              : NVFP4DG_OK;
+}
+
+}  // namespace
+}  // namespace nvfp4dg
+
+extern "C" {
+
+int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream) {
+  return nvfp4dg::run_linear(args, nullptr, nullptr, 0, false, stream);
+}
+
+int nvfp4_linear_run_grouped(const nvfp4_linear_args* args,
+                             const int* group_rows, const int* group_row0,
+                             int groups, int on_device, void* stream) {
+  nvfp4dg::host_clear_error();
+  if (groups < 1 || groups > nvfp4dg::kMaxGroups)
+    return nvfp4dg::host_fail(
+        NVFP4DG_ERR_INVALID,
+        "groups must be 1.." + std::to_string(nvfp4dg::kMaxGroups));
+  if (group_rows == nullptr)
+    return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID, "group_rows is required");
+  return nvfp4dg::run_linear(args, group_rows, group_row0, groups,
+                             on_device != 0, stream);
+}
+
+int nvfp4_linear_plan(int M, int N, int K, unsigned flags, int num_sms,
+                      int* tokens_out, int* split_out, int* grid_out) {
+  nvfp4dg::host_clear_error();
+  if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 64 || num_sms <= 0)
+    return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
+                              "invalid problem for planning");
+  const nvfp4dg::LinearPlan pl = nvfp4dg::plan_linear(
+      (M + 31) / 32, (M + 63) / 64, (M + 127) / 128, N, K, 0, flags, num_sms);
+  if (tokens_out) *tokens_out = pl.tn;
+  if (split_out) *split_out = pl.split;
+  if (grid_out) *grid_out = pl.grid;
+  return NVFP4DG_OK;
+}
+
+}  // extern "C"
