@@ -298,6 +298,7 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
 #define NVFP4DG_LINEAR_TOKENS32 (1u << 0)
 #define NVFP4DG_LINEAR_TOKENS64 (1u << 1)
 #define NVFP4DG_LINEAR_TOKENS128 (1u << 2)
+#define NVFP4DG_LINEAR_PAIR (1u << 3) /* 256 x 256 tiles of two SMs */
 #define NVFP4DG_LINEAR_SPLIT_MASK 0x700u
 #define NVFP4DG_LINEAR_SPLIT(log2) ((1u + (log2)) << 8)
 

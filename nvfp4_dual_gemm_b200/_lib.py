@@ -49,6 +49,7 @@ ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_GELU = range(5)
 LINEAR_TOKENS32 = 1 << 0
 LINEAR_TOKENS64 = 1 << 1
 LINEAR_TOKENS128 = 1 << 2
+LINEAR_PAIR = 1 << 3
 
 
 def linear_split(ctas: int) -> int:

@@ -77,13 +77,21 @@ struct LinearParams {
   int row0[kMaxGroups];
 };
 
-// Grouped products: group g owns rows [row0, row0 + rows) of A and C and
-// tiles [tile0[g], tile0[g + 1]).
+// Grouped products: group g's rows start at row0 of A and C and its tiles are
+// [tile0[g], tile0[g + 1]).
 struct GroupTable {
   int tile0[kMaxGroups + 1];
   int row0[kMaxGroups];
-  int rows[kMaxGroups];
 };
+
+// Rows of group g, whose first row lies in the matrix: its count, cut at the
+// last row.  (Read again for each tile, from L1 or the constant cache, to
+// leave shared memory to the operands.)
+__device__ __forceinline__ int group_rows(const LinearParams& p, int g,
+                                          int row0) {
+  const int n = p.dev_rows ? p.dev_rows[g] : p.rows[g];
+  return min(max(n, 0), p.M - row0);
+}
 
 struct Tile {
   int g;       // group (batch of B)
@@ -134,7 +142,6 @@ __device__ __forceinline__ void build_groups(const LinearParams& p, int tn,
     if (in) {
       tab.tile0[g] = tile_end + tiles - mine;
       tab.row0[g] = n ? static_cast<int>(r0) : 0;
-      tab.rows[g] = n;
     }
     tile_end += __shfl_sync(0xffffffffu, tiles, 31);
   }
@@ -165,13 +172,14 @@ __device__ __forceinline__ Tile locate(const LinearParams& p,
       hi = mid - 1;
   }
   const int local = tile - tab.tile0[lo];
-  const int mt = (tab.rows[lo] + TN - 1) / TN;
+  const int rows = group_rows(p, lo, tab.row0[lo]);
+  const int mt = (rows + TN - 1) / TN;
   const int nt = local / mt;
   const int m0 = (local - nt * mt) * TN;
   t.g = lo;
   t.n0 = nt * kFeat;
   t.x0 = tab.row0[lo] + m0;
-  t.rows = tab.rows[lo] - m0;
+  t.rows = rows - m0;
   return t;
 }
 
@@ -682,21 +690,564 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
+// linear_pair_kernel: many tokens.  A cluster of two CTAs computes 256 tokens
+// x 256 features with 2-SM MMAs: CTA r holds token rows [128r, 128r + 128)
+// and weight rows [128r, 128r + 128) of the tile, so an SM streams 38 KiB of
+// operands per K block for the MMAs of 54 KiB in a tile of its own, and
+// receives its 128 token rows of the accumulator.  The even CTA issues; both
+// CTAs' tiles land on its `full` barriers.  A thread of the epilogue is a
+// token row; outputs leave through shared memory and TMA stores, 64 columns
+// at a time.
+// ---------------------------------------------------------------------------
+constexpr int kPairStages = 5;
+constexpr int kPairTile = 128 * kRowBytes;  // one CTA's token or weight rows
+constexpr int kPairStageBytes = 2 * kPairTile + 3 * kRunBytes;
+constexpr int kPairSfBase = 256;   // TMEM: accumulator, then the scales
+constexpr int kPairSfCols = 48;    // 16 of tokens, 32 of weights per stage
+constexpr int kBoxBytes = 128 * 128;  // 128 rows x 64 columns of C
+constexpr int kPairSmem = kPairStages * kPairStageBytes + 2 * kBoxBytes + 1024;
+constexpr int kBand = 8;  // m tiles of a band, see locate_pair
+static_assert(kPairSmem + 4096 <= 227 * 1024, "shared memory");
+static_assert(kPairSfBase + kPairStages * kPairSfCols <= kTmemCols, "TMEM");
+
+struct PairTile {
+  int g, n0, x0, rows;  // as Tile, x0 the first of 256 token rows
+  int sfa_last;         // last row block of the scales that may be read
+};
+
+// Tiles of one problem run in bands of eight m tiles, m fastest: the tiles in
+// flight then form a block of about 8 x 9 tiles, which reads fewer distinct
+// operand rows than whole columns of m tiles do.
+__device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
+                                                const GroupTable& tab,
+                                                int tile) {
+  PairTile t;
+  if (p.groups == 0) {
+    const int per = kBand * p.n_tiles;
+    const int band = tile / per;
+    const int in = tile - band * per;
+    const int width = min(kBand, p.m_tiles - band * kBand);
+    const int nt = in / width;
+    t.g = 0;
+    t.n0 = nt * 256;
+    t.x0 = (band * kBand + in - nt * width) * 256;
+    t.rows = p.M - t.x0;
+    t.sfa_last = (p.M - 1) / 128;
+    return t;
+  }
+  int lo = 0, hi = p.groups - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tab.tile0[mid] <= tile)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  const int local = tile - tab.tile0[lo];
+  const int rows = group_rows(p, lo, tab.row0[lo]);
+  const int mt = (rows + 255) / 256;
+  const int nt = local / mt;
+  const int m0 = (local - nt * mt) * 256;
+  t.g = lo;
+  t.n0 = nt * 256;
+  t.x0 = tab.row0[lo] + m0;
+  t.rows = rows - m0;
+  t.sfa_last = (tab.row0[lo] + rows - 1) / 128;
+  return t;
+}
+
+// Barrier of the four epilogue warps, and one that also ANDs a predicate.
+__device__ __forceinline__ void epi_bar() {
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+}
+__device__ __forceinline__ bool epi_all(bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(out)
+      : "r"(static_cast<uint32_t>(pred))
+      : "memory");
+  return out != 0;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16),
+                     __uint_as_float(u & 0xFFFF0000u));
+}
+
+// Epilogue of 32 columns of one row from column n: accumulators v to packed
+// outputs o.
+template <typename T>
+__device__ __forceinline__ void finish_row32(const LinearParams& p, int x,
+                                             int n, bool live, float scale,
+                                             const float* bias, float (&v)[32],
+                                             uint4 (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 b = reinterpret_cast<const float4*>(bias)[i];
+    v[4 * i + 0] = fmaf(p.alpha, v[4 * i + 0], b.x);
+    v[4 * i + 1] = fmaf(p.alpha, v[4 * i + 1], b.y);
+    v[4 * i + 2] = fmaf(p.alpha, v[4 * i + 2], b.z);
+    v[4 * i + 3] = fmaf(p.alpha, v[4 * i + 3], b.w);
+  }
+  activate<32>(v, p.act);
+  if (p.row_scale != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= scale;
+  }
+  const T* res = p.residual == nullptr
+                     ? nullptr
+                     : static_cast<const T*>(p.residual) + (size_t)x * p.ldr;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (res != nullptr && live && n + 8 * q < p.N) {
+      const uint4 r = *reinterpret_cast<const uint4*>(res + n + 8 * q);
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<T>(w[i]);
+        v[8 * q + 2 * i] += f.x;
+        v[8 * q + 2 * i + 1] += f.y;
+      }
+    }
+    o[q].x = pack2<T>(v[8 * q + 0], v[8 * q + 1]);
+    o[q].y = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
+    o[q].z = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
+    o[q].w = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tmW,
+                       const __grid_constant__ CUtensorMap tmX,
+                       const __grid_constant__ CUtensorMap tmC,
+                       const __grid_constant__ LinearParams p) {
+  constexpr int S = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[S];
+  __shared__ __align__(8) uint64_t sfdata_bar[S];
+  __shared__ __align__(8) uint64_t empty_bar[S];
+  __shared__ __align__(8) uint64_t acc_full_bar;
+  __shared__ __align__(8) uint64_t acc_empty_bar;
+  __shared__ __align__(8) uint64_t drain_bar;
+  __shared__ uint32_t tmem_base_sh;
+  __shared__ __align__(16) float bias_sh[256];
+  __shared__ GroupTable tab;
+
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();  // 0: issues the MMAs
+  const bool leader = rank == 0;
+  const int kblk64 = p.K / 64;
+  // A K block's scale run has the same size for every block: the last
+  // block's, when K % 256 != 0, starts earlier and its first atoms are
+  // skipped (`skip` in the scale warps).
+  const uint32_t run_bytes =
+      static_cast<uint32_t>(min(4, kblk64)) * kAtomBytes;
+
+  if (warp == 0) {
+    uint64_t* bar = nullptr;
+    uint32_t count = 1;
+    if (lane < S) {
+      bar = full_bar + lane;
+      count = 2 * kSfWarps;
+    } else if (lane < 2 * S) {
+      bar = sfdata_bar + (lane - S);
+    } else if (lane < 3 * S) {
+      bar = empty_bar + (lane - 2 * S);
+    } else if (lane == 3 * S) {
+      bar = &acc_full_bar;
+    } else if (lane == 3 * S + 1) {
+      bar = &acc_empty_bar;
+      count = 2 * kEpiWarps;
+    } else if (lane == 3 * S + 2) {
+      bar = &drain_bar;
+    }
+    if (bar != nullptr) {
+      mbar_init(bar, count);
+      fence_mbar_init();
+    }
+    if (lane == 0) s_wait_failed = 0u;
+    if (lane == 29) prefetch_tmap(&tmW);
+    if (lane == 30) prefetch_tmap(&tmX);
+    if (lane == 31) prefetch_tmap(&tmC);
+    __syncwarp();
+    if (lane < S) mbar_arrive_expect_tx(sfdata_bar + lane, 3 * run_bytes);
+    fence_proxy_async_smem();
+    __syncwarp();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc_pair(&tmem_base_sh, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  cluster_arrive_relaxed();
+  griddep_launch_dependents();
+  if (p.groups > 0 && warp == 1) {
+    if (p.dev_rows != nullptr) griddep_wait();
+    build_groups(p, 256, lane, tab);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  cluster_wait();  // both CTAs' barriers are initialised
+  const uint32_t tmem = tmem_base_sh;
+  const int total =
+      p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
+  const int first = static_cast<int>(blockIdx.x) / 2;
+  const int step = static_cast<int>(gridDim.x) / 2;
+
+  if (warp == kProdWWarp || warp == kProdXWarp) {
+    // ---------------------------------------------------------- producers
+    // Warp 4: token scales, the first run of weight scales, token rows; warp
+    // 5: the second run, weight rows.  They only copy: the expected bytes
+    // come with the scale warps' arrivals.
+    if (lane == 0) {
+      const bool x_side = warp == kProdWWarp;
+      const uint64_t pol = x_side ? kPolicyEvictLast : kPolicyEvictNormal;
+      const uint32_t full_c = mapa_shared(smem_u32(&full_bar[0]), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      griddep_wait();  // global memory only after the previous grid
+      for (int tile = first; ok && tile < total; tile += step) {
+        const PairTile t = locate_pair(p, tab, tile);
+        const int row = (x_side ? t.x0 : t.n0) + 128 * static_cast<int>(rank);
+        // the odd CTA's rows may lie past the problem's last row block, and
+        // the second weight run past the last one: they copy the last, whose
+        // products are never stored
+        const uint8_t* sfa =
+            p.sfa + (size_t)min(t.x0 / 128 + static_cast<int>(rank),
+                                t.sfa_last) *
+                        kblk64 * kAtomBytes;
+        const int nb = t.n0 / 128 + (x_side ? 0 : 1);
+        const uint8_t* sfb = p.sfb + (size_t)t.g * p.sfb_group +
+                             (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
+                                 kAtomBytes;
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (issued >= S &&
+              !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
+                                 kErrProducer)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + stage * kPairStageBytes;
+          uint8_t* sf = st + 2 * kPairTile;
+          const size_t run =
+              (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes;
+          const uint32_t full_s = full_c + 8u * static_cast<uint32_t>(stage);
+          if (x_side) {
+            // the MMAs that read this stage in both CTAs are done: pass that
+            // on to the odd CTA
+            if (leader && issued >= S)
+              mbar_arrive_cluster(mapa_shared(smem_u32(&empty_bar[stage]), 1));
+            bulk_load(sf, sfa + run, run_bytes, &sfdata_bar[stage], pol);
+            bulk_load(sf + kRunBytes, sfb + run, run_bytes,
+                      &sfdata_bar[stage], pol);
+            tma_load_3d_pair(st, &tmX, full_s, kb * kRowBytes, row, 0, pol);
+          } else {
+            bulk_load(sf + 2 * kRunBytes, sfb + run, run_bytes,
+                      &sfdata_bar[stage], pol);
+            tma_load_3d_pair(st + kPairTile, &tmW, full_s, kb * kRowBytes,
+                             row, t.g, pol);
+          }
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // never leave with copies in flight: scale runs land on this CTA's
+      // barriers, both CTAs' tiles on the even one's
+      for (int s = 0; s < S; ++s) {
+        if (issued > s) {
+          const uint32_t par =
+              static_cast<uint32_t>(((issued - 1 - s) / S) & 1);
+          mbar_wait(&sfdata_bar[s], par, p.err, kErrDrain, false);
+          if (x_side && leader)
+            mbar_wait_cluster(&full_bar[s], par, p.err, kErrDrain, false);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kSfWarp0) {
+    // ---------------------------------------------------------- scale warps
+    const uint32_t q = static_cast<uint32_t>(warp % 4);
+    const uint32_t t_lane = tmem + ((32u * q) << 16);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    griddep_wait();
+    for (int tile = first; ok && tile < total; tile += step) {
+      for (int kb = 0; kb < p.kblocks; ++kb) {
+        const bool got = mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
+        }
+        // arm the stage's next fill: it cannot complete before all four
+        // scale warps have passed this one
+        if (warp == kSfWarp0 && lane == 0)
+          mbar_arrive_expect_tx(&sfdata_bar[stage], 3 * run_bytes);
+        const int skip = 4 * kb - min(4 * kb, max(0, kblk64 - 4));
+        const uint32_t sf_s =
+            smem_u32(smem + stage * kPairStageBytes + 2 * kPairTile) +
+            16u * lane;
+        const uint32_t col = t_lane + kPairSfBase + stage * kPairSfCols;
+        uint32_t ra[16], rb[32];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // (past the run for the steps of a short block that are not issued)
+          const uint32_t at = sf_s + min(j + skip, 3) * kAtomBytes;
+          const uint4 v = lds128(at);
+          const uint4 w0 = lds128(at + kRunBytes);
+          const uint4 w1 = lds128(at + 2 * kRunBytes);
+          ra[4 * j + 0] = v.x;
+          ra[4 * j + 1] = v.y;
+          ra[4 * j + 2] = v.z;
+          ra[4 * j + 3] = v.w;
+          rb[8 * j + 0] = w0.x;
+          rb[8 * j + 1] = w0.y;
+          rb[8 * j + 2] = w0.z;
+          rb[8 * j + 3] = w0.w;
+          rb[8 * j + 4] = w1.x;
+          rb[8 * j + 5] = w1.y;
+          rb[8 * j + 6] = w1.z;
+          rb[8 * j + 7] = w1.w;
+        }
+        __syncwarp();
+        tc_st_16cols(col, ra);
+        tc_st_32cols(col + 16, rb);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t full_s = mapa_shared(smem_u32(&full_bar[stage]), 0);
+          if (leader && warp == kSfWarp0)
+            mbar_arrive_expect_tx_cluster(full_s, 4 * kPairTile);
+          else
+            mbar_arrive_cluster(full_s);
+        }
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------- MMA issuer
+    if (lane == 0 && leader) {
+      constexpr uint32_t kIdesc = idesc_nvf4(256, 256);
+      const uint64_t x_desc0 =
+          smem_desc(smem_u32(smem), 16, 1024, SmemLayout::kSwizzle128B);
+      const uint64_t w_desc0 = smem_desc(smem_u32(smem) + kPairTile, 16, 1024,
+                                         SmemLayout::kSwizzle128B);
+      int stage = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true, any = false;
+      for (int tile = first; ok && tile < total; tile += step) {
+        if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
+                               kErrMma)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t soff =
+              static_cast<uint32_t>(stage) * (kPairStageBytes >> 4);
+          const uint32_t sf_t = tmem + kPairSfBase + stage * kPairSfCols;
+          const uint32_t acc0 = kb > 0 ? 1u : 0u;
+          if (4 * kb + 4 <= kblk64) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
+                               w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
+                               sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
+          } else {
+            for (int j = 0; j < kblk64 - 4 * kb; ++j)
+              tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
+                               w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
+                               sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
+          }
+          tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 0));
+          any = true;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(mapa_shared(smem_u32(&acc_full_bar), 0));
+        tc_commit_pair(mapa_shared(smem_u32(&acc_full_bar), 1));
+        acc_phase ^= 1u;
+      }
+      // the last release of the accumulator (the odd CTA's warps arrive here
+      // remotely) is awaited like the others, so that no arrival is in
+      // flight when the CTAs leave
+      if (ok && any)
+        mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err, kErrMma);
+      tc_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
+      mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
+    }
+    __syncwarp();
+  } else {
+    // ---------------------------------------------------------- epilogue
+    const int row = threadIdx.x;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t acc_empty_c = mapa_shared(smem_u32(&acc_empty_bar), 0);
+    uint8_t* boxes = smem + S * kPairStageBytes;
+    uint32_t acc_phase = 0;
+    int stores = 0;  // boxes stored, alternately
+    griddep_wait();
+    for (int tile = first; tile < total; tile += step, acc_phase ^= 1u) {
+      const PairTile t = locate_pair(p, tab, tile);
+      const int rows = t.rows - 128 * static_cast<int>(rank);  // of this CTA
+      const int x = t.x0 + 128 * static_cast<int>(rank) + row;
+      const bool live = row < rows;
+      const float scale =
+          p.row_scale != nullptr && live ? p.row_scale[x] : 0.f;
+      epi_bar();  // the previous tile's bias has been read
+      bias_sh[row] = load_bias<T>(p, t.g, t.n0 + row);
+      bias_sh[row + 128] = load_bias<T>(p, t.g, t.n0 + row + 128);
+      const bool got =
+          mbar_wait_cluster(&acc_full_bar, acc_phase, p.err, kErrEpilogue);
+      // the four warps leave together: they meet at the barriers below
+      if (!epi_all(got)) break;
+      tc_fence_after();
+      // a group's last rows are stored row by row: a box would overwrite the
+      // rows behind them
+      const bool boxed = p.groups == 0 ? rows > 0 : rows >= 128;
+#pragma unroll 1
+      for (int ph = 0; ph < 4; ++ph) {
+        float v[2][32];
+        __syncwarp();
+        tc_ld_32cols(t_row + 64 * ph, v[0]);
+        tc_ld_32cols(t_row + 64 * ph + 32, v[1]);
+        tc_wait_ld();
+        tie32(v[0]);
+        tie32(v[1]);
+        if (ph == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_empty_c);
+        }
+        const int n = t.n0 + 64 * ph;
+        if (n >= p.N) continue;
+        uint8_t* box = boxes + (stores & 1) * kBoxBytes;
+        if (boxed) {
+          // the store before last read this box
+          if (threadIdx.x == 0)
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          epi_bar();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint4 o[4];
+          finish_row32<T>(p, x, n + 32 * h, live, scale,
+                          bias_sh + 64 * ph + 32 * h, v[h], o);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (boxed)
+              sts128(smem_u32(box + row * 128 +
+                              (((4 * h + q) ^ (row & 7)) << 4)),
+                     o[q]);
+            else if (live && n + 32 * h + 8 * q < p.N)
+              *reinterpret_cast<uint4*>(static_cast<T*>(p.C) +
+                                        (size_t)x * p.ldc + n + 32 * h +
+                                        8 * q) = o[q];
+          }
+        }
+        if (boxed) {
+          fence_proxy_async_smem();
+          epi_bar();
+          if (threadIdx.x == 0) {
+            tma_store_2d(&tmC, box, 2 * n, t.x0 + 128 * static_cast<int>(rank));
+            bulk_commit_group();
+          }
+          ++stores;
+        }
+      }
+    }
+    // the stores must have read their boxes before shared memory goes away
+    if (threadIdx.x == 0) bulk_wait_group_read0();
+    __syncwarp();
+  }
+
+  // ------------------------------------------------------------ teardown
+  tc_fence_before();
+  cluster_sync_final();  // no CTA leaves while its peer may still signal it
+  if (warp == kMmaWarp) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
 struct LinearPlan {
-  int tn;      // tokens per tile
+  int tn;      // tokens per tile (256: 2-SM pairs)
   int split;   // CTAs that share a tile's K range
   int grid;    // CTAs
   int tiles;
 };
 
-LinearPlan plan_linear(long long m_tiles32, long long m_tiles64,
-                       long long m_tiles128, int N, int K, int groups,
+// `mt`: token tiles of 32, 64, 128 and 256 tokens (of all groups).
+LinearPlan plan_linear(const long long (&mts)[4], int N, int K, int groups,
                        unsigned flags, int sms) {
   LinearPlan pl{};
   const int n_tiles = (N + kFeat - 1) / kFeat;
   const int kblocks = (K + 255) / 256;
+  const long long pair_tiles = mts[3] * ((N + 255) / 256);
+  const unsigned forced_tile =
+      flags & (NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
+               NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR);
+  const long long units = sms / 2;
+  // waves of tiles, each by its K blocks' time
+  const double pair_cost =
+      double((pair_tiles + units - 1) / units) * (kblocks * 620.0 + 2500);
+  const double one_cost =
+      double((mts[2] * n_tiles + sms - 1) / sms) * (kblocks * 560.0 + 1500);
+  if (sms >= 2 && ((flags & NVFP4DG_LINEAR_PAIR) ||
+                   (!forced_tile && mts[2] > mts[3] && pair_cost < one_cost))) {
+    pl.tn = 256;
+    pl.split = 1;
+    pl.tiles = static_cast<int>(std::min<long long>(pair_tiles, 1 << 30));
+    pl.grid = 2 * static_cast<int>(std::min<long long>(pair_tiles, units));
+    return pl;
+  }
   // the narrowest tile that holds as few tiles as the widest: columns beyond
   // the tokens cost shared memory and MMA time
   if (flags & NVFP4DG_LINEAR_TOKENS32)
@@ -706,9 +1257,8 @@ LinearPlan plan_linear(long long m_tiles32, long long m_tiles64,
   else if (flags & NVFP4DG_LINEAR_TOKENS128)
     pl.tn = 128;
   else
-    pl.tn = m_tiles32 == m_tiles128 ? 32 : m_tiles64 == m_tiles128 ? 64 : 128;
-  const long long mt =
-      pl.tn == 32 ? m_tiles32 : pl.tn == 64 ? m_tiles64 : m_tiles128;
+    pl.tn = mts[0] == mts[2] ? 32 : mts[1] == mts[2] ? 64 : 128;
+  const long long mt = pl.tn == 32 ? mts[0] : pl.tn == 64 ? mts[1] : mts[2];
   pl.tiles = static_cast<int>(std::min<long long>(mt * n_tiles, 1 << 30));
   pl.split = 1;
   const int forced =
@@ -771,6 +1321,42 @@ int launch_linear(const LinearParams& kp, const LinearPlan& pl,
   return NVFP4DG_OK;
 }
 
+template <typename T>
+int launch_pair(const LinearParams& kp, const LinearPlan& pl,
+                const CUtensorMap& tw, const CUtensorMap& tx,
+                const CUtensorMap& tc, int dev, unsigned flags,
+                cudaStream_t stream) {
+  static std::atomic<unsigned long long> ready{0};
+  auto kernel = linear_pair_kernel<T>;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(ready.load() & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
+    ready.fetch_or(bit);
+  }
+  LinearParams p = kp;
+  p.m_tiles = (p.M + 255) / 256;
+  p.n_tiles = (p.N + 255) / 256;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = 2;
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = (flags & NVFP4DG_FLAG_NO_PDL) ? 1 : 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tw, tx, tc, p);
+  if (e != cudaSuccess) return host_cuda_fail(e, "linear_pair_kernel launch");
+  return NVFP4DG_OK;
+}
+
 int check_linear(const nvfp4_linear_args* a, int groups,
                  bool placed_on_device) {
   if (a == nullptr) return host_fail(NVFP4DG_ERR_INVALID, "args is NULL");
@@ -790,11 +1376,13 @@ int check_linear(const nvfp4_linear_args* a, int groups,
     return host_fail(NVFP4DG_ERR_INVALID, "unknown activation");
   const unsigned t = a->flags & (NVFP4DG_LINEAR_TOKENS32 |
                                  NVFP4DG_LINEAR_TOKENS64 |
-                                 NVFP4DG_LINEAR_TOKENS128);
+                                 NVFP4DG_LINEAR_TOKENS128 |
+                                 NVFP4DG_LINEAR_PAIR);
   if (t & (t - 1))
-    return host_fail(NVFP4DG_ERR_INVALID, "the TOKENS flags are exclusive");
+    return host_fail(NVFP4DG_ERR_INVALID, "the tile flags are exclusive");
   const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
-                         NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_SPLIT_MASK |
+                         NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR |
+                         NVFP4DG_LINEAR_SPLIT_MASK |
                          NVFP4DG_FLAG_SYNC_CHECK | NVFP4DG_FLAG_NO_PDL;
   if (a->flags & ~known)
     return host_fail(NVFP4DG_ERR_INVALID, "unknown flag bits");
@@ -845,7 +1433,7 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
   LinearParams p;
   std::memset(&p, 0, sizeof(p));
-  long long mt[3] = {0, 0, 0};
+  long long mt[4] = {0, 0, 0, 0};
   if (groups > 0 && !on_device) {
     long long next = 0;
     for (int g = 0; g < groups; ++g) {
@@ -872,6 +1460,7 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
       mt[0] += (n + 31) / 32;
       mt[1] += (n + 63) / 64;
       mt[2] += (n + 127) / 128;
+      mt[3] += (n + 255) / 256;
     }
     if (mt[0] == 0) return NVFP4DG_OK;
   } else {
@@ -881,12 +1470,14 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
     mt[0] = (per + 31) / 32 * g;
     mt[1] = (per + 63) / 64 * g;
     mt[2] = (per + 127) / 128 * g;
+    mt[3] = (per + 255) / 256 * g;
   }
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
-  LinearPlan pl = plan_linear(mt[0], mt[1], mt[2], a->N, a->K, groups,
-                              a->flags, dev.sms);
-  if (groups > 0 && on_device) pl.grid = dev.sms;
+  LinearPlan pl = plan_linear(mt, a->N, a->K, groups, a->flags, dev.sms);
+  // tiles counted by the kernel: a full grid
+  if (groups > 0 && on_device)
+    pl.grid = pl.tn == 256 ? dev.sms / 2 * 2 : dev.sms;
   p.M = a->M;
   p.N = a->N;
   p.K = a->K;
@@ -914,11 +1505,21 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   if ((rc = host_byte_map(a->B, a->N, kb, kb, kFeat, std::max(groups, 1),
                           a->N * kb, &tw)))
     return rc;
-  if ((rc = host_byte_map(a->A, a->M, kb, kb, pl.tn, 1, a->M * kb, &tx)))
+  if ((rc = host_byte_map(a->A, a->M, kb, kb, std::min(pl.tn, 128), 1,
+                          a->M * kb, &tx)))
     return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const bool bf = a->c_dtype == NVFP4DG_DTYPE_BF16;
-  if (pl.tn == 32)
+  if (pl.tn == 256) {
+    CUtensorMap tc;
+    if ((rc = host_byte_map(a->C, a->M, 2ll * a->N, 2 * a->ldc, 128, 0, 0,
+                            &tc)))
+      return rc;
+    rc = bf ? launch_pair<__nv_bfloat16>(p, pl, tw, tx, tc, dev.id, a->flags,
+                                         stream)
+            : launch_pair<__half>(p, pl, tw, tx, tc, dev.id, a->flags,
+                                  stream);
+  } else if (pl.tn == 32)
     rc = bf ? launch_linear<__nv_bfloat16, 32>(p, pl, tw, tx, dev.id,
                                                a->flags, stream)
             : launch_linear<__half, 32>(p, pl, tw, tx, dev.id, a->flags,
@@ -967,8 +1568,10 @@ int nvfp4_linear_plan(int M, int N, int K, unsigned flags, int num_sms,
   if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 64 || num_sms <= 0)
     return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
                               "invalid problem for planning");
-  const nvfp4dg::LinearPlan pl = nvfp4dg::plan_linear(
-      (M + 31) / 32, (M + 63) / 64, (M + 127) / 128, N, K, 0, flags, num_sms);
+  const long long mts[4] = {(M + 31ll) / 32, (M + 63ll) / 64,
+                            (M + 127ll) / 128, (M + 255ll) / 256};
+  const nvfp4dg::LinearPlan pl =
+      nvfp4dg::plan_linear(mts, N, K, 0, flags, num_sms);
   if (tokens_out) *tokens_out = pl.tn;
   if (split_out) *split_out = pl.split;
   if (grid_out) *grid_out = pl.grid;

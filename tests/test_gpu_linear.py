@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 
 SYNC = _lib.FLAG_SYNC_CHECK
 TILES = {"auto": 0, "t32": _lib.LINEAR_TOKENS32, "t64": _lib.LINEAR_TOKENS64,
-         "t128": _lib.LINEAR_TOKENS128}
+         "t128": _lib.LINEAR_TOKENS128, "pair": _lib.LINEAR_PAIR}
 
 
 def dev(x):
@@ -67,6 +67,7 @@ def test_every_schedule(m, n, k, tile, split):
 def test_rows(m):
     p = Problem(m, 200, 512, seed=m)
     p.check(p.run(), f"m {m}")
+    p.check(p.run(flags=_lib.LINEAR_PAIR), f"pair, m {m}")
 
 
 @pytest.mark.parametrize("n", [8, 16, 72, 120, 128, 136, 256, 1000])
@@ -74,6 +75,7 @@ def test_rows(m):
 def test_columns(m, n):
     p = Problem(m, n, 320, seed=n, residual=True)
     p.check(p.run(), f"n {n}")
+    p.check(p.run(flags=_lib.LINEAR_PAIR), f"pair, n {n}")
 
 
 @pytest.mark.parametrize("k", [64, 128, 192, 256, 320, 448, 512, 1088, 4096])
@@ -81,15 +83,17 @@ def test_columns(m, n):
 def test_depth(m, k):
     p = Problem(m, 144, k, seed=k)
     p.check(p.run(), f"k {k}")
+    p.check(p.run(flags=_lib.LINEAR_PAIR), f"pair, k {k}")
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("act", [None, "relu", "silu", "gelu_tanh", "gelu"])
-@pytest.mark.parametrize("m", [7, 150])
+@pytest.mark.parametrize("m", [7, 150, 300])
 def test_epilogue(m, act, dtype):
     p = Problem(m, 264, 384, seed=5, dtype=dtype, bias=dtype, residual=True,
                 row_scale=True)
-    got = p.run(dtype=dtype, activation=act, alpha=0.375)
+    got = p.run(dtype=dtype, activation=act, alpha=0.375,
+                flags=_lib.LINEAR_PAIR if m == 300 else 0)
     p.check(got, f"{act}", act=act, alpha=0.375)
 
 
@@ -98,9 +102,12 @@ def test_many_tiles_per_cta():
     p = Problem(700, 4360, 576, seed=9, residual=True)
     p.check(p.run(flags=_lib.LINEAR_TOKENS32 | _lib.linear_split(1)))
     p.check(p.run(flags=_lib.LINEAR_TOKENS128 | _lib.linear_split(1)))
+    p = Problem(2100, 4360, 576, seed=10, residual=True, bias=torch.float32)
+    p.check(p.run(flags=_lib.LINEAR_PAIR))
 
 
-def test_output_given_strided_and_in_place():
+@pytest.mark.parametrize("tile", ["auto", "pair"])
+def test_output_given_strided_and_in_place(tile):
     m, n, k = 45, 200, 256
     p = Problem(m, n, k, seed=3, residual=True)
     wide = torch.full((m, n + 56), float("nan"), dtype=torch.float16,
@@ -108,7 +115,7 @@ def test_output_given_strided_and_in_place():
     wide[:, 8:n + 8] = p.kw["residual"]
     view = wide[:, 8:n + 8]
     p.kw["residual"] = view
-    out = p.run(C=view)  # residual and output are the same strided rows
+    out = p.run(C=view, flags=TILES[tile])  # residual and output are the same strided rows
     assert out.data_ptr() == view.data_ptr()
     p.check(view, "in place")
     assert torch.isnan(wide[:, :8]).all() and torch.isnan(wide[:, n + 8:]).all()
