@@ -14,7 +14,9 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "host.h"
 #include "nvfp4_dual_gemm.h"
@@ -25,151 +27,295 @@ namespace nvfp4dg {
 namespace {
 
 constexpr int kAtomBytes = 512;  // scales of 128 rows x 64 elements
+constexpr int kMaxDepth = 8;     // rows a CTA has in flight
 
 struct NormParams {
   nvfp4_block_norm_args a;
   int gate_run;  // rows of one gate row
   int rows_pad;  // rows whose scales are written (NVFP4 output), else rows
+  int depth;     // rows in flight (block_norm_rows_kernel)
+  unsigned* err;
 };
 
-// Eight consecutive elements as fp32.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    using H2 = typename std::conditional<std::is_same<T, __half>::value,
-                                         __half2, __nv_bfloat162>::type;
-    v[2 * i] = Half2Ops<H2>::lo(w[i]);
-    v[2 * i + 1] = Half2Ops<H2>::hi(w[i]);
-  }
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p);
-  const float4 b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// The four scales of 64 elements of a row in the blocked layout.
+__device__ __forceinline__ uint32_t* scale_word(const nvfp4_block_norm_args& a,
+                                                int row, int g) {
+  return reinterpret_cast<uint32_t*>(
+      static_cast<uint8_t*>(a.sf) +
+      ((size_t)(row / 128) * (a.D / 64) + g) * kAtomBytes + (row % 32) * 16 +
+      ((row % 128) / 32) * 4);
 }
 
-// Rounds eight values to T: `w` gets the bits to store, v the values.
+// ---------------------------------------------------------------------------
+// Vectors of eight consecutive elements.  The arithmetic runs on pairs of
+// fp32 values (fma.rn.f32x2 and its like): at 16 bits an element the kernels
+// are bound by instructions before they are by memory.
+// ---------------------------------------------------------------------------
+struct F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 template <typename T>
-struct Round8 {
-  uint32_t w[4];
-  __device__ __forceinline__ void set(float (&v)[8]) {
+using Pair = typename std::conditional<std::is_same<T, __half>::value,
+                                       __half2, __nv_bfloat162>::type;
+
+// As loaded: the bits.
+template <typename T>
+struct Raw8 {
+  uint32_t w[sizeof(T) * 2];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4* s = reinterpret_cast<const uint4*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        v[2 * i] = Half2Ops<__half2>::lo(w[i]);
-        v[2 * i + 1] = Half2Ops<__half2>::hi(w[i]);
-      } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        v[2 * i] = Half2Ops<__nv_bfloat162>::lo(w[i]);
-        v[2 * i + 1] = Half2Ops<__nv_bfloat162>::hi(w[i]);
-      }
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      const uint4 u = s[i];
+      w[4 * i] = u.x;
+      w[4 * i + 1] = u.y;
+      w[4 * i + 2] = u.z;
+      w[4 * i + 3] = u.w;
     }
   }
-  __device__ __forceinline__ uint32_t word(int i) const { return w[i]; }
   __device__ __forceinline__ void store(T* p) const {
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <>
-struct Round8<float> {
-  float f[8];
-  __device__ __forceinline__ void set(float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = v[i];
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(
+          w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
-  __device__ __forceinline__ uint32_t word(int i) const {
-    return __float_as_uint(f[i]);
+  __device__ __forceinline__ F2 pair(int i) const {  // elements 2i, 2i + 1
+    if constexpr (sizeof(T) == 4)
+      return {__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1])};
+    else
+      return {Half2Ops<Pair<T>>::lo(w[i]), Half2Ops<Pair<T>>::hi(w[i])};
   }
-  __device__ __forceinline__ void store(float* p) const {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  __device__ __forceinline__ void set(int i, F2 v) {  // rounds
+    if constexpr (sizeof(T) == 4) {
+      w[2 * i] = __float_as_uint(v.x);
+      w[2 * i + 1] = __float_as_uint(v.y);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2 h = __floats2half2_rn(v.x, v.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
   }
 };
 
+struct V8 {
+  F2 p[4];
+};
+
+// A norm's weight or bias at vector j.
 template <typename T>
-__device__ __forceinline__ void load_w8(const void* w, int w_f32, int i,
-                                        float (&v)[8]) {
-  if (w_f32)
-    load8<float>(static_cast<const float*>(w) + i, v);
-  else
-    load8<T>(static_cast<const T*>(w) + i, v);
+__device__ __forceinline__ V8 load_param(const void* src, int f32, int j) {
+  V8 v;
+  if (f32) {
+    Raw8<float> r;
+    r.load(static_cast<const float*>(src) + 8 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.p[i] = r.pair(i);
+  } else {
+    Raw8<T> r;
+    r.load(static_cast<const T*>(src) + 8 * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.p[i] = r.pair(i);
+  }
+  return v;
 }
 
-// Sum over the threads of a row: a warp (WARP_ROW) or the whole CTA.  `slot`
-// is a shared buffer of 32 words that the row's previous sum did not use.
-template <bool WARP_ROW>
-__device__ __forceinline__ float row_sum(float v, float* slot) {
+// One parameter vector of a thread's columns (vector t + i * threads).  HELD
+// loads it at the kernel's start, so that its latency hides behind the row's;
+// otherwise it is read where it is used (from L1, for a CTA of many rows).
+template <typename T, int VPT, bool HELD>
+struct Param {
+  const void* src;
+  int f32;
+  V8 v[HELD ? VPT : 1];
+  __device__ __forceinline__ void set(const void* s, int is_f32, int vecs,
+                                      int t, int threads) {
+    src = s;
+    f32 = is_f32;
+    if (HELD && src != nullptr) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (WARP_ROW) return v;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  if (lane == 0) slot[warp] = v;
-  __syncthreads();
-  v = lane < static_cast<int>(blockDim.x) / 32 ? slot[lane] : 0.f;
+      for (int i = 0; i < VPT; ++i)
+        if (t + i * threads < vecs)
+          v[i] = load_param<T>(src, f32, t + i * threads);
+    }
+  }
+  __device__ __forceinline__ V8 get(int i, int j) const {
+    return HELD ? v[i] : load_param<T>(src, f32, j);
+  }
+};
+
+template <typename T, int VPT, bool HELD, bool HELD_BIAS>
+struct Params {
+  Param<T, VPT, HELD> weight, post_weight;
+  Param<T, VPT, HELD_BIAS> bias, post_bias;
+  __device__ __forceinline__ void set(const nvfp4_block_norm_args& a,
+                                      int vecs, int t, int threads) {
+    const int f32 = a.w_dtype == NVFP4DG_DTYPE_F32;
+    post_weight.set(a.post_weight, f32, vecs, t, threads);
+    post_bias.set(a.post_bias, f32, vecs, t, threads);
+    weight.set(a.weight, f32, vecs, t, threads);
+    bias.set(a.bias, f32, vecs, t, threads);
+  }
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
   return v;
 }
 
-// v <- norm(v) * w + b over a row of D elements, VPT vectors of eight a
-// thread (vector t + i * threads).  The layer norm's variance is summed from
-// the centred values, not as a difference of large sums.
-template <typename T, int VPT, bool WARP_ROW>
-__device__ __forceinline__ void norm_row(float (&v)[VPT][8], int vecs, int t,
-                                         int threads, int D, int kind,
-                                         float eps, const void* w,
-                                         const void* b, int w_f32,
-                                         float* slots) {
-  if (kind == NVFP4DG_NORM_LAYER) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (t + i * threads < vecs) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s += v[i][k];
-      }
-    const float mean = row_sum<WARP_ROW>(s, slots) / D;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] -= mean;
-  }
-  float q = 0.f;
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (t + i * threads < vecs) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) q = fmaf(v[i][k], v[i][k], q);
-    }
-  const float inv = rsqrtf(row_sum<WARP_ROW>(q, slots + 32) / D + eps);
+// A row's vectors of one thread: f(i, j) for vector j = t + i * threads.
+template <int VPT, typename F>
+__device__ __forceinline__ void each(int vecs, int t, int threads, F f) {
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int j = t + i * threads;
-    if (j < vecs) {
-      float f[8];
-      if (w != nullptr) {
-        load_w8<T>(w, w_f32, 8 * j, f);
+    if (j < vecs) f(i, j);
+  }
+}
+
+// inv = 1 / sqrt(mean(v^2) + eps) of each of NR rows v, which a layer norm
+// centres first; v leaves multiplied by the norm's weight.  A row lies in a
+// warp (WARP_ROW) or in the whole CTA, whose warps exchange their sums through
+// `slots` (64 floats a row that no thread still reads from) and one barrier.
+// A layer norm's warps each sum the squares about their own mean; with n
+// values of sum s and such a square sum q in a warp, the row's are
+// sum(q + n (s / n - mean)^2) about the row's mean (Chan, Golub and LeVeque,
+// 1979), so nothing is a difference of large sums.
+template <bool WARP_ROW, bool LAYER, int NR, int VPT, typename P>
+__device__ __forceinline__ void norm_factors(V8 (&v)[NR][VPT], int vecs,
+                                             int t, int threads, int D,
+                                             float eps, const P& w,
+                                             float* slots,
+                                             float (&inv)[NR]) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warps = threads / 32;
+  float s[NR], q[NR];
+  if (LAYER) {
+    // values of warp l's threads
+    auto count = [&](int l) {
+      int n = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] * inv * f[k];
-      } else {
+      for (int i = 0; i < VPT; ++i)
+        n += min(32, max(0, vecs - i * threads - 32 * l)) * 8;
+      return n;
+    };
+    const int own = WARP_ROW ? D : count(warp);
+    const float per = own > 0 ? 1.f / own : 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] *= inv;
+    for (int r = 0; r < NR; ++r) {
+      F2 a = {0.f, 0.f};
+      each<VPT>(vecs, t, threads, [&](int i, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a = add2(a, v[r][i].p[k]);
+      });
+      s[r] = warp_sum(a.x + a.y);
+    }
+    float mean[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const float m = mean[r] = -s[r] * per;
+      F2 a = {0.f, 0.f};
+      each<VPT>(vecs, t, threads, [&](int i, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const F2 c = add2(v[r][i].p[k], {m, m});
+          a = fma2(c, c, a);
+        }
+      });
+      q[r] = warp_sum(a.x + a.y);
+    }
+    if (!WARP_ROW) {
+      if (lane == 0) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          slots[64 * r + warp] = s[r];
+          slots[64 * r + 32 + warp] = q[r];
+        }
       }
-      if (b != nullptr) {
-        load_w8<T>(b, w_f32, 8 * j, f);
+      __syncthreads();
+      const float n = lane < warps ? static_cast<float>(count(lane)) : 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] += f[k];
+      for (int r = 0; r < NR; ++r) {
+        const float sl = lane < warps ? slots[64 * r + lane] : 0.f;
+        const float ql = lane < warps ? slots[64 * r + 32 + lane] : 0.f;
+        mean[r] = -warp_sum(sl) / D;
+        const float d = n > 0.f ? sl / n + mean[r] : 0.f;
+        q[r] = warp_sum(fmaf(n * d, d, ql));
       }
     }
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+      each<VPT>(vecs, t, threads, [&](int i, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[r][i].p[k] = add2(v[r][i].p[k], {mean[r], mean[r]});
+      });
+  } else {
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      F2 a = {0.f, 0.f};
+      each<VPT>(vecs, t, threads, [&](int i, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a = fma2(v[r][i].p[k], v[r][i].p[k], a);
+      });
+      q[r] = a.x + a.y;
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) q[r] = warp_sum(q[r]);
+    if (!WARP_ROW && lane == 0) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) slots[64 * r + warp] = q[r];
+    }
   }
+  if (w.src != nullptr)
+    each<VPT>(vecs, t, threads, [&](int i, int j) {
+      const V8 f = w.get(i, j);
+#pragma unroll
+      for (int r = 0; r < NR; ++r)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[r][i].p[k] = mul2(v[r][i].p[k], f.p[k]);
+    });
+  if (!LAYER && !WARP_ROW) {
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < NR; ++r)
+      q[r] = lane < warps ? slots[64 * r + lane] : 0.f;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) q[r] = warp_sum(q[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) inv[r] = rsqrtf(q[r] / D + eps);
 }
 
 // One half (eight values, rounded to T) of a 16-element block whose other
@@ -177,15 +323,16 @@ __device__ __forceinline__ void norm_row(float (&v)[VPT][8], int vecs, int t,
 // scale byte, as the activation quantiser's (quant.cuh).  All lanes of a warp
 // call it.
 template <typename T>
-__device__ __forceinline__ uint32_t quant_half(const float (&v)[8],
-                                               const Round8<T>& z,
-                                               uint8_t& sb) {
+__device__ __forceinline__ uint32_t quant_half(const Raw8<T>& z, uint8_t& sb) {
   uint32_t x[8], key = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = __float_as_uint(v[i]);
-    key = max(key, x[i] & 0x7FFFFFFFu);
+  for (int i = 0; i < 4; ++i) {
+    const F2 v = z.pair(i);
+    x[2 * i] = __float_as_uint(v.x);
+    x[2 * i + 1] = __float_as_uint(v.y);
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) key = max(key, x[i] & 0x7FFFFFFFu);
   key = max(key, __shfl_xor_sync(0xffffffffu, key, 1));
   const float amax = __uint_as_float(key);
   sb = __nv_cvt_float_to_fp8(amax / 6.0f, __NV_SATFINITE, __NV_E4M3);
@@ -194,11 +341,11 @@ __device__ __forceinline__ uint32_t quant_half(const float (&v)[8],
   // a block holding a NaN goes to the compare form, which takes all sixteen
   if (__any_sync(0xffffffffu, key > 0x7F800000u)) {
     const bool hi = threadIdx.x & 1;
-    constexpr int kWords = sizeof(T) == 2 ? 4 : 8;
+    constexpr int kWords = sizeof(T) * 2;
     uint32_t f[2 * kWords];
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-      const uint32_t own = z.word(i);
+      const uint32_t own = z.w[i];
       const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
       f[i] = hi ? other : own;
       f[kWords + i] = hi ? own : other;
@@ -206,9 +353,7 @@ __device__ __forceinline__ uint32_t quant_half(const float (&v)[8],
     if (key > 0x7F800000u) {
       uint32_t w0, w1;
       if constexpr (sizeof(T) == 2) {
-        using H2 = typename std::conditional<std::is_same<T, __half>::value,
-                                             __half2, __nv_bfloat162>::type;
-        sb = quant_block16_x2_cmp<H2>(f, w0, w1);
+        sb = quant_block16_x2_cmp<Pair<T>>(f, w0, w1);
       } else {
         float e[16];
 #pragma unroll
@@ -221,7 +366,121 @@ __device__ __forceinline__ uint32_t quant_half(const float (&v)[8],
   return w;
 }
 
-template <typename T, int VPT, bool WARP_ROW, int MAXT>
+// NR rows from `row` (the first `live` of them exist): v holds y (x where there
+// is no y); x(r, i, j) and gate(r, i, j) give those vectors when they are
+// needed; `consumed` runs once every thread of the rows has asked for all.
+template <typename T, bool WARP_ROW, bool LAYER, int NR, int VPT, typename P,
+          typename X, typename G, typename C>
+__device__ __forceinline__ void finish_rows(const nvfp4_block_norm_args& a,
+                                            const P& w, int row, int live,
+                                            int vecs, int t, int threads,
+                                            V8 (&v)[NR][VPT], X x, G gate,
+                                            C consumed, float* slots) {
+  float inv[NR];
+  if (a.y != nullptr) {
+    float s[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) s[r] = a.scale;
+    if (a.post) {
+      norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.D, a.eps,
+                                             w.post_weight, slots, inv);
+      if (w.post_bias.src != nullptr)
+        each<VPT>(vecs, t, threads, [&](int i, int j) {
+          const V8 b = w.post_bias.get(i, j);
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              v[r][i].p[k] = fma2(v[r][i].p[k], {inv[r], inv[r]}, b.p[k]);
+        });
+      else
+#pragma unroll
+        for (int r = 0; r < NR; ++r) s[r] *= inv[r];
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      T* R = static_cast<T*>(a.R) + (size_t)(row + r) * a.ldr;
+      each<VPT>(vecs, t, threads, [&](int i, int j) {
+        if (a.gate != nullptr) {
+          const Raw8<T> g = gate(r, i, j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[r][i].p[k] = mul2(v[r][i].p[k], g.pair(k));
+        }
+        const Raw8<T> xr = x(r, i, j);
+        Raw8<T> o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          o.set(k, fma2(v[r][i].p[k], {s[r], s[r]}, xr.pair(k)));
+          v[r][i].p[k] = o.pair(k);
+        }
+        if (r < live) o.store(R + 8 * j);
+      });
+    }
+  }
+  if (a.Z == nullptr && a.codes == nullptr) {
+    if (!WARP_ROW) __syncthreads();
+    consumed();
+    return;
+  }
+  norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.D, a.eps,
+                                         w.weight, slots + 64 * NR, inv);
+  consumed();  // after the barrier of the sums
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = t + i * threads;
+    const bool in = j < vecs;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      Raw8<T> z;
+      if (in) {
+        if (w.bias.src != nullptr) {
+          const V8 b = w.bias.get(i, j);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            z.set(k, fma2(v[r][i].p[k], {inv[r], inv[r]}, b.p[k]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            z.set(k, mul2(v[r][i].p[k], {inv[r], inv[r]}));
+        }
+        if (a.Z != nullptr && r < live)
+          z.store(static_cast<T*>(a.Z) + (size_t)(row + r) * a.ldz + 8 * j);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z.set(k, {0.f, 0.f});
+      }
+      if (a.codes == nullptr) continue;
+      uint8_t sb;
+      const uint32_t c = quant_half<T>(z, sb);
+      if (in && r < live)
+        *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.codes) +
+                                     (size_t)(row + r) * (a.D / 2) + 4 * j) =
+            c;
+      // the eight lanes of 64 elements hold four scales, each twice
+      const uint32_t s1 = __shfl_down_sync(0xffffffffu, sb, 2);
+      const uint32_t s2 = __shfl_down_sync(0xffffffffu, sb, 4);
+      const uint32_t s3 = __shfl_down_sync(0xffffffffu, sb, 6);
+      if ((j & 7) == 0 && in && r < live)
+        *scale_word(a, row + r, j / 8) =
+            static_cast<uint32_t>(sb) | (s1 << 8) | (s2 << 16) | (s3 << 24);
+    }
+  }
+}
+
+template <typename T, int VPT>
+__device__ __forceinline__ void unpack_row(const Raw8<T> (&r)[VPT],
+                                           V8 (&v)[VPT]) {
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[i].p[k] = r[i].pair(k);
+}
+
+// One row for each warp (WARP_ROW) or CTA: rows of up to 1024 elements, and
+// wider ones when there are too few to go round.  Every load is issued before
+// the first sum.
+template <typename T, int VPT, bool WARP_ROW, bool LAYER, int MAXT>
 __global__ void __launch_bounds__(MAXT)
     block_norm_kernel(const __grid_constant__ NormParams p) {
   __shared__ float slots[128];
@@ -232,120 +491,239 @@ __global__ void __launch_bounds__(MAXT)
                            : blockIdx.x;
   griddep_launch_dependents();
   griddep_wait();
-  if (row >= p.rows_pad) return;
   const int vecs = a.D / 8;
-  const int w_f32 = a.w_dtype == NVFP4DG_DTYPE_F32;
-  const bool live = row < a.rows;
-  float r[VPT][8];
-  if (live) {
-    float u[VPT][8];
-    const T* x = static_cast<const T*>(a.x) + (size_t)row * a.ldx;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = t + i * threads;
-      if (j < vecs) load8<T>(x + 8 * j, r[i]);
-    }
-    if (a.y != nullptr) {
-      const T* y = static_cast<const T*>(a.y) + (size_t)row * a.ldy;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int j = t + i * threads;
-        if (j < vecs) load8<T>(y + 8 * j, u[i]);
-      }
-      if (a.post)
-        norm_row<T, VPT, WARP_ROW>(u, vecs, t, threads, a.D, a.kind, a.eps,
-                                   a.post_weight, a.post_bias, w_f32, slots);
-      const T* g = a.gate ? static_cast<const T*>(a.gate) +
-                                (size_t)(row / p.gate_run) * a.D
-                          : nullptr;
-      T* R = static_cast<T*>(a.R) + (size_t)row * a.ldr;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int j = t + i * threads;
-        if (j < vecs) {
-          if (g != nullptr) {
-            float f[8];
-            load8<T>(g + 8 * j, f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) u[i][k] *= f[k];
-          }
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            r[i][k] = fmaf(a.scale, u[i][k], r[i][k]);
-          Round8<T> o;
-          o.set(r[i]);
-          o.store(R + 8 * j);
-        }
-      }
-    }
-    if (a.Z == nullptr && a.codes == nullptr) return;
-    norm_row<T, VPT, WARP_ROW>(r, vecs, t, threads, a.D, a.kind, a.eps,
-                               a.weight, a.bias, w_f32, slots + 64);
+  if (row >= a.rows) {
+    if (row < p.rows_pad)
+      for (int g = t; g < vecs / 8; g += threads) *scale_word(a, row, g) = 0u;
+    return;
   }
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int j = t + i * threads;
-    const bool in = live && j < vecs;
-    Round8<T> z;
-    if (in) {
-      z.set(r[i]);
-      if (a.Z != nullptr)
-        z.store(static_cast<T*>(a.Z) + (size_t)row * a.ldz + 8 * j);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r[i][k] = 0.f;
-      z.set(r[i]);
-    }
-    if (a.codes == nullptr) continue;
-    uint8_t sb;
-    const uint32_t w = quant_half<T>(r[i], z, sb);
-    if (in)
-      *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.codes) +
-                                   (size_t)row * (a.D / 2) + 4 * j) = w;
-    // the eight lanes of 64 elements hold four scales, each twice
-    const uint32_t s1 = __shfl_down_sync(0xffffffffu, sb, 2);
-    const uint32_t s2 = __shfl_down_sync(0xffffffffu, sb, 4);
-    const uint32_t s3 = __shfl_down_sync(0xffffffffu, sb, 6);
-    if ((j & 7) == 0 && j < vecs)
-      *reinterpret_cast<uint32_t*>(
-          static_cast<uint8_t*>(a.sf) +
-          ((size_t)(row / 128) * (a.D / 64) + j / 8) * kAtomBytes +
-          (row % 32) * 16 + ((row % 128) / 32) * 4) =
-          static_cast<uint32_t>(sb) | (s1 << 8) | (s2 << 16) | (s3 << 24);
-  }
+  Raw8<T> x[VPT], y[VPT], g[VPT];
+  each<VPT>(vecs, t, threads, [&](int i, int j) {
+    x[i].load(static_cast<const T*>(a.x) + (size_t)row * a.ldx + 8 * j);
+    if (a.y != nullptr)
+      y[i].load(static_cast<const T*>(a.y) + (size_t)row * a.ldy + 8 * j);
+    if (a.gate != nullptr)
+      g[i].load(static_cast<const T*>(a.gate) +
+                (size_t)(row / p.gate_run) * a.D + 8 * j);
+  });
+  Params<T, VPT, VPT == 1, VPT == 1> w;
+  w.set(a, vecs, t, threads);
+  V8 v[1][VPT];
+  if (a.y != nullptr)
+    unpack_row<T, VPT>(y, v[0]);
+  else
+    unpack_row<T, VPT>(x, v[0]);
+  finish_rows<T, WARP_ROW, LAYER, 1, VPT>(
+      a, w, row, 1, vecs, t, threads, v, [&](int, int i, int) { return x[i]; },
+      [&](int, int i, int) { return g[i]; }, [] {}, slots);
 }
 
-template <typename T>
-int launch_norm(const NormParams& p, int sms, cudaStream_t stream) {
-  const int vecs = p.a.D / 8;
-  void (*kernel)(NormParams);
-  int threads, grid;
-  if (vecs <= 128) {  // a warp holds the row
-    threads = p.rows_pad >= 4 * sms ? 256 : 64;
-    grid = (p.rows_pad + threads / 32 - 1) / (threads / 32);
-    kernel = vecs <= 32   ? block_norm_kernel<T, 1, true, 256>
-             : vecs <= 64 ? block_norm_kernel<T, 2, true, 256>
-                          : block_norm_kernel<T, 4, true, 256>;
-  } else {
-    grid = p.rows_pad;
-    const int vpt = vecs <= 512 ? 1 : vecs <= 1024 ? 2 : 4;
-    threads = ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
-    kernel = vpt == 1   ? block_norm_kernel<T, 1, false, 512>
-             : vpt == 2 ? block_norm_kernel<T, 2, false, 512>
-                        : block_norm_kernel<T, 4, false, 1024>;
+// Many wide rows: a CTA works through pairs of rows, and bulk copies bring the
+// next pairs of x, y (and of a gate that differs from row to row) into shared
+// memory while it computes: the copies in flight do not depend on how many
+// warps wait in a row's sums.  A thread holds one vector of both rows, so that
+// each barrier serves two sums, and the norms' weights stay in its registers.
+constexpr int kPairRows = 2;
+
+template <typename T, bool LAYER, int MAXT, int CTAS>
+__global__ void __launch_bounds__(MAXT, CTAS)
+    block_norm_rows_kernel(const __grid_constant__ NormParams p) {
+  constexpr int NR = kPairRows;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float slots[2][128 * NR];
+  __shared__ __align__(8) uint64_t full_bar[kMaxDepth];
+  const nvfp4_block_norm_args& a = p.a;
+  const int t = threadIdx.x, threads = blockDim.x;
+  const int vecs = a.D / 8;
+  const uint32_t row_bytes = a.D * sizeof(T);
+  const bool gate_rows = a.gate != nullptr && a.gate_rows > 1;
+  const uint32_t srcs = 1 + (a.y != nullptr) + gate_rows;
+  const uint32_t stage_bytes = NR * srcs * row_bytes;
+  if (t == 0) {
+    for (int i = 0; i < kMaxDepth; ++i) mbar_init(&full_bar[i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    s_wait_failed = 0u;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
+  griddep_launch_dependents();
+  __syncthreads();
+  griddep_wait();
+  // a stage: for each row y (where there is one), x and the gate; behind the
+  // last row the last row again
+  auto fetch = [&](int pair, int stage) {  // thread 0
+    uint8_t* dst = ring + stage * stage_bytes;
+    uint64_t* bar = &full_bar[stage];
+    mbar_arrive_expect_tx(bar, stage_bytes);
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      const int row = min(pair * NR + r, a.rows - 1);
+      if (a.y != nullptr) {
+        bulk_load(dst, static_cast<const T*>(a.y) + (size_t)row * a.ldy,
+                  row_bytes, bar, kPolicyEvictFirst);
+        dst += row_bytes;
+      }
+      bulk_load(dst, static_cast<const T*>(a.x) + (size_t)row * a.ldx,
+                row_bytes, bar, kPolicyEvictFirst);
+      dst += row_bytes;
+      if (gate_rows) {
+        bulk_load(dst,
+                  static_cast<const T*>(a.gate) +
+                      (size_t)(row / p.gate_run) * a.D,
+                  row_bytes, bar, kPolicyEvictNormal);
+        dst += row_bytes;
+      }
+    }
+  };
+  const int stride = gridDim.x;
+  const int pairs = (a.rows + NR - 1) / NR;
+  int ahead = blockIdx.x;  // thread 0: next pair to fetch
+  if (t == 0) {
+    for (int i = 0; i < p.depth && ahead < pairs; ++i, ahead += stride)
+      fetch(ahead, i);
+  }
+  Params<T, 1, true, false> w;
+  w.set(a, vecs, t, threads);
+  int stage = 0, it = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  for (int pair = blockIdx.x; pair < pairs; pair += stride, ++it) {
+    // (after a wait that ran out the values are stale, every access is in
+    // bounds and the error word reports it; the sums' barriers are still met)
+    ok = mbar_wait(&full_bar[stage], phase, p.err, kErrProducer) && ok;
+    const T* src = reinterpret_cast<const T*>(ring + stage * stage_bytes);
+    const uint32_t x_at = a.y != nullptr ? a.D : 0;
+    V8 v[NR][1];
+    if (t < vecs) {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        Raw8<T> u;
+        u.load(src + r * srcs * a.D + 8 * t);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[r][0].p[k] = u.pair(k);
+      }
+    }
+    finish_rows<T, false, LAYER, NR, 1>(
+        a, w, pair * NR, min(NR, a.rows - pair * NR), vecs, t, threads, v,
+        [&](int r, int, int j) {
+          Raw8<T> u;
+          u.load(src + r * srcs * a.D + x_at + 8 * j);
+          return u;
+        },
+        [&](int r, int, int j) {
+          Raw8<T> u;
+          u.load(gate_rows ? src + (r + 1) * srcs * a.D - a.D + 8 * j
+                           : static_cast<const T*>(a.gate) + 8 * j);
+          return u;
+        },
+        [&] {
+          if (t == 0 && ahead < pairs && ok) {
+            fence_proxy_async_smem();  // the reads, before the refill
+            fetch(ahead, stage);
+            ahead += stride;
+          }
+        },
+        slots[it & 1]);
+    if (++stage == p.depth) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  // after a wait that ran out, copies may be in flight: let them land
+  if (t == 0 && !ok) {
+    const int n = (ahead - static_cast<int>(blockIdx.x)) / stride;
+    for (int i = max(0, n - p.depth); i < n; ++i)
+      mbar_wait(&full_bar[i % p.depth], (i / p.depth) & 1, p.err, kErrDrain,
+                /*bail_on_err=*/false);
+  }
+  for (int row = a.rows + blockIdx.x; row < p.rows_pad; row += stride)
+    for (int g = t; g < vecs / 8; g += threads) *scale_word(a, row, g) = 0u;
+}
+
+// Bytes of a stage of block_norm_rows_kernel, and the most it may use.
+int rows_stage(const nvfp4_block_norm_args& a, int elem) {
+  const int srcs = 1 + (a.y != nullptr) +
+                   (a.gate != nullptr && a.gate_rows > 1);
+  return kPairRows * srcs * a.D * elem;
+}
+constexpr int kRowsSmem = 216 * 1024;
+
+template <typename T, bool LAYER, int MAXT, int CTAS>
+int launch_rows(NormParams p, int sms, int dev, int threads,
+                cudaLaunchConfig_t& cfg) {
+  static std::atomic<unsigned long long> ready{0};
+  static std::atomic<int> regs{0};
+  auto kernel = block_norm_rows_kernel<T, LAYER, MAXT, CTAS>;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(ready.load() & bit)) {
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncGetAttributes");
+    regs = (fa.numRegs + 7) / 8 * 8;
+    e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
+    ready.fetch_or(bit);
+  }
+  // CTAs an SM holds by its registers (a persistent grid must fit at once)
+  // and with two stages or more each
+  const int stage = rows_stage(p.a, sizeof(T));
+  int ctas =
+      std::min(65536 / (regs.load() * threads), kRowsSmem / (2 * stage));
+  ctas = std::max(1, std::min(ctas, 8));
+  p.depth = std::min(kMaxDepth, (kRowsSmem / ctas - 2048) / stage);
+  cfg.gridDim = dim3(std::min((p.a.rows + 1) / 2, sms * ctas), 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.depth) * stage;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess)
+    return host_cuda_fail(e, "block_norm_rows_kernel launch");
+  return NVFP4DG_OK;
+}
+
+template <typename T, bool LAYER>
+int launch_norm(const NormParams& p, int sms, int dev, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = (p.a.flags & NVFP4DG_FLAG_NO_PDL) ? 0 : 1;
+  const int vecs = p.a.D / 8;
+  auto cover = [&](int vpt) {  // threads of vpt vectors each
+    return ((vecs + vpt - 1) / vpt + 31) / 32 * 32;
+  };
+  void (*kernel)(NormParams);
+  if (vecs <= 128) {  // a warp holds the row
+    const int threads = p.rows_pad >= 4 * sms ? 256 : 64;
+    cfg.gridDim = dim3((p.rows_pad + threads / 32 - 1) / (threads / 32), 1, 1);
+    cfg.blockDim = dim3(threads, 1, 1);
+    kernel = vecs <= 32   ? block_norm_kernel<T, 1, true, LAYER, 256>
+             : vecs <= 64 ? block_norm_kernel<T, 2, true, LAYER, 256>
+                          : block_norm_kernel<T, 4, true, LAYER, 256>;
+  } else {
+    if (p.a.rows > 2 * sms && vecs <= 1024 &&
+        rows_stage(p.a, sizeof(T)) <= kRowsSmem - 2048)
+      return vecs <= 512
+                 ? launch_rows<T, LAYER, 512, 2>(p, sms, dev, cover(1), cfg)
+                 : launch_rows<T, LAYER, 1024, 1>(p, sms, dev, cover(1), cfg);
+    const int vpt = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+    cfg.gridDim = dim3(p.rows_pad, 1, 1);
+    cfg.blockDim = dim3(cover(vpt), 1, 1);
+    kernel = vpt == 1   ? block_norm_kernel<T, 1, false, LAYER, 1024>
+             : vpt == 2 ? block_norm_kernel<T, 2, false, LAYER, 1024>
+                        : block_norm_kernel<T, 4, false, LAYER, 1024>;
+  }
   cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) return host_cuda_fail(e, "block_norm_kernel launch");
   return NVFP4DG_OK;
+}
+
+template <typename T>
+int launch_norm(const NormParams& p, int sms, int dev, cudaStream_t stream) {
+  return p.a.kind == NVFP4DG_NORM_LAYER
+             ? launch_norm<T, true>(p, sms, dev, stream)
+             : launch_norm<T, false>(p, sms, dev, stream);
 }
 
 int check_norm(const nvfp4_block_norm_args* a) {
@@ -419,8 +797,12 @@ extern "C" int nvfp4_block_norm_run(const nvfp4_block_norm_args* a,
   p.a = *a;
   p.gate_run = a->gate != nullptr ? a->rows / a->gate_rows : 1;
   p.rows_pad = a->codes != nullptr ? (a->rows + 127) / 128 * 128 : a->rows;
+  p.depth = 0;
+  p.err = dev.err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == NVFP4DG_DTYPE_F32) return launch_norm<float>(p, dev.sms, s);
-  if (a->dtype == NVFP4DG_DTYPE_F16) return launch_norm<__half>(p, dev.sms, s);
-  return launch_norm<__nv_bfloat16>(p, dev.sms, s);
+  if (a->dtype == NVFP4DG_DTYPE_F32)
+    return launch_norm<float>(p, dev.sms, dev.id, s);
+  if (a->dtype == NVFP4DG_DTYPE_F16)
+    return launch_norm<__half>(p, dev.sms, dev.id, s);
+  return launch_norm<__nv_bfloat16>(p, dev.sms, dev.id, s);
 }
