@@ -203,34 +203,79 @@ __device__ __forceinline__ void each(int vecs, int t, int threads, F f) {
   }
 }
 
+// Sums over a warp of NR values a lane.  Of two values, each half of the warp
+// takes one after the first exchange (five shuffles for both, not ten): lanes
+// [0, 16) return the first sum and lanes [16, 32) the second.
+template <int NR>
+__device__ __forceinline__ float warp_sums(const float (&v)[NR], int lane) {
+  if (NR == 1) return warp_sum(v[0]);
+  const bool hi = lane >= 16;
+  float s = (hi ? v[NR - 1] : v[0]) +
+            __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[NR - 1], 16);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+// Value of row r in the layout warp_sums returns.
+template <int NR>
+__device__ __forceinline__ float pick(float v, int r) {
+  return NR == 1 ? v : __shfl_sync(0xffffffffu, v, 16 * r);
+}
+
+// What a thread knows of its rows' sums: the part of the warps' sums it adds
+// up after the barrier.  With two rows, each half warp adds one row's.
+template <bool WARP_ROW, int NR>
+struct Sums {
+  int lane, warp, part;      // part: this lane's row
+  float per_row, per_warp;   // 1 / values of a row, of this warp
+  float n[NR], per[NR];      // values of the warps this lane adds up, and 1 / n
+  template <int VPT>
+  __device__ __forceinline__ void set(int vecs, int threads, int D) {
+    lane = threadIdx.x % 32;
+    warp = threadIdx.x / 32;
+    part = NR == 1 ? 0 : lane / 16;
+    per_row = 1.f / D;
+    auto count = [&](int l) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i)
+        c += min(32, max(0, min(vecs - i * threads, threads) - 32 * l)) * 8;
+      return c;
+    };
+    const int own = WARP_ROW ? D : count(warp);
+    per_warp = own > 0 ? 1.f / own : 0.f;
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+      const int c = count(other(k));
+      n[k] = c;
+      per[k] = c > 0 ? 1.f / c : 0.f;
+    }
+  }
+  // the k-th warp this lane adds up: 32 warps over 32 or 16 lanes
+  __device__ __forceinline__ int other(int k) const {
+    return NR == 1 ? lane : (lane & 15) + 16 * k;
+  }
+};
+
 // inv = 1 / sqrt(mean(v^2) + eps) of each of NR rows v, which a layer norm
 // centres first; v leaves multiplied by the norm's weight.  A row lies in a
 // warp (WARP_ROW) or in the whole CTA, whose warps exchange their sums through
-// `slots` (64 floats a row that no thread still reads from) and one barrier.
-// A layer norm's warps each sum the squares about their own mean; with n
-// values of sum s and such a square sum q in a warp, the row's are
-// sum(q + n (s / n - mean)^2) about the row's mean (Chan, Golub and LeVeque,
-// 1979), so nothing is a difference of large sums.
+// `slots` (64 floats a row that no thread still reads from, zero behind the
+// last warp) and one barrier.  A layer norm's warps each sum the squares about
+// their own mean; with n values of sum s and such a square sum q in a warp,
+// the row's are sum(q + n (s / n - mean)^2) about the row's mean (Chan, Golub
+// and LeVeque, 1979), so nothing is a difference of large sums.
 template <bool WARP_ROW, bool LAYER, int NR, int VPT, typename P>
 __device__ __forceinline__ void norm_factors(V8 (&v)[NR][VPT], int vecs,
-                                             int t, int threads, int D,
-                                             float eps, const P& w,
+                                             int t, int threads, float eps,
+                                             const P& w,
+                                             const Sums<WARP_ROW, NR>& u,
                                              float* slots,
                                              float (&inv)[NR]) {
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int warps = threads / 32;
-  float s[NR], q[NR];
+  float s[NR], q[NR], ws = 0.f, wq;
+  const bool writes = !WARP_ROW && (u.lane & (NR == 1 ? 31 : 15)) == 0;
+  float* mine = slots + 64 * u.part;
   if (LAYER) {
-    // values of warp l's threads
-    auto count = [&](int l) {
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        n += min(32, max(0, vecs - i * threads - 32 * l)) * 8;
-      return n;
-    };
-    const int own = WARP_ROW ? D : count(warp);
-    const float per = own > 0 ? 1.f / own : 0.f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       F2 a = {0.f, 0.f};
@@ -238,84 +283,81 @@ __device__ __forceinline__ void norm_factors(V8 (&v)[NR][VPT], int vecs,
 #pragma unroll
         for (int k = 0; k < 4; ++k) a = add2(a, v[r][i].p[k]);
       });
-      s[r] = warp_sum(a.x + a.y);
+      s[r] = a.x + a.y;
     }
-    float mean[NR];
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      const float m = mean[r] = -s[r] * per;
-      F2 a = {0.f, 0.f};
-      each<VPT>(vecs, t, threads, [&](int i, int) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const F2 c = add2(v[r][i].p[k], {m, m});
-          a = fma2(c, c, a);
-        }
-      });
-      q[r] = warp_sum(a.x + a.y);
-    }
-    if (!WARP_ROW) {
-      if (lane == 0) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          slots[64 * r + warp] = s[r];
-          slots[64 * r + 32 + warp] = q[r];
-        }
-      }
-      __syncthreads();
-      const float n = lane < warps ? static_cast<float>(count(lane)) : 0.f;
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        const float sl = lane < warps ? slots[64 * r + lane] : 0.f;
-        const float ql = lane < warps ? slots[64 * r + 32 + lane] : 0.f;
-        mean[r] = -warp_sum(sl) / D;
-        const float d = n > 0.f ? sl / n + mean[r] : 0.f;
-        q[r] = warp_sum(fmaf(n * d, d, ql));
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-      each<VPT>(vecs, t, threads, [&](int i, int) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          v[r][i].p[k] = add2(v[r][i].p[k], {mean[r], mean[r]});
-      });
-  } else {
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      F2 a = {0.f, 0.f};
-      each<VPT>(vecs, t, threads, [&](int i, int) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a = fma2(v[r][i].p[k], v[r][i].p[k], a);
-      });
-      q[r] = a.x + a.y;
-    }
-#pragma unroll
-    for (int r = 0; r < NR; ++r) q[r] = warp_sum(q[r]);
-    if (!WARP_ROW && lane == 0) {
-#pragma unroll
-      for (int r = 0; r < NR; ++r) slots[64 * r + warp] = q[r];
-    }
+    ws = warp_sums<NR>(s, u.lane);
   }
-  if (w.src != nullptr)
-    each<VPT>(vecs, t, threads, [&](int i, int j) {
-      const V8 f = w.get(i, j);
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
+  for (int r = 0; r < NR; ++r) {
+    const float m = LAYER ? -pick<NR>(ws, r) * u.per_warp : 0.f;
+    F2 a = {0.f, 0.f};
+    each<VPT>(vecs, t, threads, [&](int i, int) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          v[r][i].p[k] = mul2(v[r][i].p[k], f.p[k]);
+      for (int k = 0; k < 4; ++k) {
+        const F2 c = LAYER ? add2(v[r][i].p[k], {m, m}) : v[r][i].p[k];
+        a = fma2(c, c, a);
+      }
     });
-  if (!LAYER && !WARP_ROW) {
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < NR; ++r)
-      q[r] = lane < warps ? slots[64 * r + lane] : 0.f;
-#pragma unroll
-    for (int r = 0; r < NR; ++r) q[r] = warp_sum(q[r]);
+    q[r] = a.x + a.y;
   }
+  wq = warp_sums<NR>(q, u.lane);
+  if (writes) {
+    mine[u.warp] = wq;
+    if (LAYER) mine[32 + u.warp] = ws;
+  }
+  auto weigh = [&] {
+    if (w.src != nullptr)
+      each<VPT>(vecs, t, threads, [&](int i, int j) {
+        const V8 f = w.get(i, j);
 #pragma unroll
-  for (int r = 0; r < NR; ++r) inv[r] = rsqrtf(q[r] / D + eps);
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[r][i].p[k] = mul2(v[r][i].p[k], f.p[k]);
+      });
+  };
+  if (!LAYER) weigh();  // under the barrier's wait
+  float mean = -ws * u.per_row;
+  if (!WARP_ROW) {
+    __syncthreads();
+    auto across = [&](float x) {  // over the lanes of one row
+#pragma unroll
+      for (int d = NR == 1 ? 16 : 8; d > 0; d >>= 1)
+        x += __shfl_xor_sync(0xffffffffu, x, d);
+      return x;
+    };
+    float sl[NR];
+    wq = 0.f;
+    if (LAYER) {
+      ws = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) ws += sl[k] = mine[32 + u.other(k)];
+      mean = -across(ws) * u.per_row;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        const float d = fmaf(sl[k], u.per[k], mean);
+        wq += fmaf(u.n[k] * d, d, mine[u.other(k)]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NR; ++k) wq += mine[u.other(k)];
+    }
+    wq = across(wq);
+  }
+  const float f = rsqrtf(fmaf(wq, u.per_row, eps));
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    inv[r] = pick<NR>(f, r);
+    if (LAYER) {
+      const float m = pick<NR>(mean, r);
+      each<VPT>(vecs, t, threads, [&](int i, int) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          v[r][i].p[k] = add2(v[r][i].p[k], {m, m});
+      });
+    }
+  }
+  if (LAYER) weigh();
 }
 
 // One half (eight values, rounded to T) of a 16-element block whose other
@@ -375,15 +417,17 @@ __device__ __forceinline__ void finish_rows(const nvfp4_block_norm_args& a,
                                             const P& w, int row, int live,
                                             int vecs, int t, int threads,
                                             V8 (&v)[NR][VPT], X x, G gate,
-                                            C consumed, float* slots) {
+                                            C consumed,
+                                            const Sums<WARP_ROW, NR>& sums,
+                                            float* slots) {
   float inv[NR];
   if (a.y != nullptr) {
     float s[NR];
 #pragma unroll
     for (int r = 0; r < NR; ++r) s[r] = a.scale;
     if (a.post) {
-      norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.D, a.eps,
-                                             w.post_weight, slots, inv);
+      norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.eps,
+                                             w.post_weight, sums, slots, inv);
       if (w.post_bias.src != nullptr)
         each<VPT>(vecs, t, threads, [&](int i, int j) {
           const V8 b = w.post_bias.get(i, j);
@@ -423,8 +467,8 @@ __device__ __forceinline__ void finish_rows(const nvfp4_block_norm_args& a,
     consumed();
     return;
   }
-  norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.D, a.eps,
-                                         w.weight, slots + 64 * NR, inv);
+  norm_factors<WARP_ROW, LAYER, NR, VPT>(v, vecs, t, threads, a.eps, w.weight,
+                                         sums, slots + 64 * NR, inv);
   consumed();  // after the barrier of the sums
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -490,6 +534,10 @@ __global__ void __launch_bounds__(MAXT)
   const int row = WARP_ROW ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32
                            : blockIdx.x;
   griddep_launch_dependents();
+  if (!WARP_ROW) {
+    for (int i = t; i < 128; i += threads) slots[i] = 0.f;
+    __syncthreads();
+  }
   griddep_wait();
   const int vecs = a.D / 8;
   if (row >= a.rows) {
@@ -497,6 +545,8 @@ __global__ void __launch_bounds__(MAXT)
       for (int g = t; g < vecs / 8; g += threads) *scale_word(a, row, g) = 0u;
     return;
   }
+  Sums<WARP_ROW, 1> sums;
+  sums.template set<VPT>(vecs, threads, a.D);
   Raw8<T> x[VPT], y[VPT], g[VPT];
   each<VPT>(vecs, t, threads, [&](int i, int j) {
     x[i].load(static_cast<const T*>(a.x) + (size_t)row * a.ldx + 8 * j);
@@ -515,7 +565,7 @@ __global__ void __launch_bounds__(MAXT)
     unpack_row<T, VPT>(x, v[0]);
   finish_rows<T, WARP_ROW, LAYER, 1, VPT>(
       a, w, row, 1, vecs, t, threads, v, [&](int, int i, int) { return x[i]; },
-      [&](int, int i, int) { return g[i]; }, [] {}, slots);
+      [&](int, int i, int) { return g[i]; }, [] {}, sums, slots);
 }
 
 // Many wide rows: a CTA works through pairs of rows, and bulk copies bring the
@@ -545,6 +595,7 @@ __global__ void __launch_bounds__(MAXT, CTAS)
     fence_proxy_async_smem();
     s_wait_failed = 0u;
   }
+  for (int i = t; i < 2 * 128 * NR; i += threads) slots[0][i] = 0.f;
   griddep_launch_dependents();
   __syncthreads();
   griddep_wait();
@@ -581,6 +632,8 @@ __global__ void __launch_bounds__(MAXT, CTAS)
     for (int i = 0; i < p.depth && ahead < pairs; ++i, ahead += stride)
       fetch(ahead, i);
   }
+  Sums<false, NR> sums;
+  sums.template set<1>(vecs, threads, a.D);
   Params<T, 1, true, false> w;
   w.set(a, vecs, t, threads);
   int stage = 0, it = 0;
@@ -622,7 +675,7 @@ __global__ void __launch_bounds__(MAXT, CTAS)
             ahead += stride;
           }
         },
-        slots[it & 1]);
+        sums, slots[it & 1]);
     if (++stage == p.depth) {
       stage = 0;
       phase ^= 1u;
