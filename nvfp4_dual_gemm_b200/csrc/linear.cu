@@ -183,6 +183,22 @@ __device__ __forceinline__ Tile locate(const LinearParams& p,
   return t;
 }
 
+// Whether the phase has completed, without waiting.  A wait on a barrier takes
+// ~300 cycles even when its phase is already complete, so each role asks for
+// its next stage before it works on the present one and waits only when the
+// answer was no: without that a K block took ~750 cycles whatever its size.
+__device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // 4 consecutive 32-bit TMEM columns of this warp's 32 lanes.
 __device__ __forceinline__ void tc_ld_4cols(uint32_t taddr, float (&v)[4]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -340,16 +356,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x % 32;
   const int S = p.stages;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int kblk64 = p.K / 64;
+  // A K block's scale run has the same size for every block: the last
+  // block's, when K % 256 != 0, starts earlier and its first atoms are
+  // skipped (`skip` in the scale warps).
+  const uint32_t run_bytes =
+      static_cast<uint32_t>(min(4, kblk64)) * kAtomBytes;
 
   if (warp == 0) {
     uint64_t* bar = nullptr;
     uint32_t count = 1;
     if (lane < 8) {
       bar = full_bar + lane;
-      count = 2 + kSfWarps;  // both producers and the scale warps
+      count = kSfWarps;  // the first one's arrival carries the tiles' bytes
     } else if (lane < 16) {
       bar = sfdata_bar + (lane - 8);
-      count = 2;
     } else if (lane < 24) {
       bar = empty_bar + (lane - 16);
     } else if (lane < 26) {
@@ -369,6 +390,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 30) prefetch_tmap(&tmW);
     if (lane == 31) prefetch_tmap(&tmX);
     if (lane == 0) s_wait_failed = 0u;
+    __syncwarp();
+    // the first scale fill of every stage; later ones are armed by the scale
+    // warps (bytes may land before their arming)
+    if (lane < S) mbar_arrive_expect_tx(sfdata_bar + lane, 2 * run_bytes);
     fence_proxy_async_smem();
     __syncwarp();
   }
@@ -396,22 +421,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kb0 = static_cast<int>((long long)p.kblocks * rank / p.split);
   const int kb1 =
       static_cast<int>((long long)p.kblocks * (rank + 1) / p.split);
-  const int kblk64 = p.K / 64;
 
   if (warp == kProdWWarp || warp == kProdXWarp) {
     // ---------------------------------------------------------- producers
+    // They only copy: a thread's instructions on barriers and copies take
+    // ~105 cycles each, and with the arming of both barriers in this loop a K
+    // block took ~1000 cycles whatever its size.
     if (lane == 0) {
       const bool w_side = warp == kProdWWarp;
       const CUtensorMap* tm = w_side ? &tmW : &tmX;
       const uint64_t pol = w_side ? kPolicyEvictNormal : kPolicyEvictLast;
-      const uint32_t tile_bytes = w_side ? Cf::kWBytes : Cf::kXBytes;
       const uint32_t tile_off = w_side ? 0 : Cf::kWBytes;
       const uint32_t sf_off =
           Cf::kWBytes + Cf::kXBytes + (w_side ? 0 : kRunBytes);
       int stage = 0;
       uint32_t phase = 0;
       long long issued = 0;
-      bool ok = true;
+      bool ok = true, ready = false;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
         const Tile t = locate<TN>(p, tab, tile);
@@ -422,26 +448,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row = w_side ? t.n0 : t.x0;
         const int layer = w_side ? t.g : 0;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (issued >= S &&
+          if (issued >= S && !ready &&
               !mbar_wait(&empty_bar[stage], phase ^ 1u, p.err,
                          kErrProducer)) {
             ok = false;
             break;
           }
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          ready = mbar_peek(&empty_bar[next], next_phase ^ 1u);
           uint8_t* st = smem + stage * Cf::kStageBytes;
-          const uint32_t run =
-              static_cast<uint32_t>(min(4, kblk64 - 4 * kb)) * kAtomBytes;
-          mbar_arrive_expect_tx(&sfdata_bar[stage], run);
-          bulk_load(st + sf_off, sf + (size_t)kb * kRunBytes, run,
-                    &sfdata_bar[stage], pol);
-          mbar_arrive_expect_tx(&full_bar[stage], tile_bytes);
+          bulk_load(st + sf_off,
+                    sf + (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes,
+                    run_bytes, &sfdata_bar[stage], pol);
           tma_load_3d(st + tile_off, tm, &full_bar[stage], kb * kRowBytes,
                       row, layer, pol);
           ++issued;
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
       }
       // never leave with copies in flight
@@ -464,25 +488,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + ((32u * q) << 16);
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
+    bool ok = true, ready = false;
     griddep_wait();
     for (int tile = first; ok && tile < total; tile += step) {
       const int part =
           TN == 128 ? 0 : (locate<TN>(p, tab, tile).x0 % 128) / 32;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const bool got = mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
+        if (!__all_sync(0xffffffffu, ready)) {
+          const bool got =
+              mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
+          if (!__all_sync(0xffffffffu, got)) {
+            ok = false;
+            break;
+          }
         }
+        const int next = stage + 1 == S ? 0 : stage + 1;
+        const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+        ready = mbar_peek(&sfdata_bar[next], next_phase);
+        // arm the stage's next fill: it cannot complete before all four
+        // scale warps have passed this one
+        if (warp == kSfWarp0 && lane == 0)
+          mbar_arrive_expect_tx(&sfdata_bar[stage], 2 * run_bytes);
+        const int skip = 4 * kb - min(4 * kb, max(0, kblk64 - 4));
         const uint32_t sf_s = smem_u32(smem + stage * Cf::kStageBytes +
                                        Cf::kWBytes + Cf::kXBytes) +
                               16u * lane;
         uint32_t r[32];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint4 w = lds128(sf_s + j * kAtomBytes);
-          const uint4 x = lds128(sf_s + kRunBytes + j * kAtomBytes);
+          // (past the run for the steps of a short block that are not issued)
+          const uint32_t at = sf_s + min(j + skip, 3) * kAtomBytes;
+          const uint4 w = lds128(at);
+          const uint4 x = lds128(at + kRunBytes);
           r[4 * j + 0] = w.x;
           r[4 * j + 1] = w.y;
           r[4 * j + 2] = w.z;
@@ -506,11 +543,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_bar[stage]);
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
+        if (lane == 0) {
+          if (warp == kSfWarp0)
+            mbar_arrive_expect_tx(&full_bar[stage],
+                                  Cf::kWBytes + Cf::kXBytes);
+          else
+            mbar_arrive(&full_bar[stage]);
         }
+        stage = next;
+        phase = next_phase;
       }
     }
   } else if (warp == kMmaWarp) {
@@ -524,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       int it = 0;
-      bool ok = true;
+      bool ok = true, ready = false;
       for (int tile = first; ok && tile < total; tile += step, ++it) {
         const int a = it & 1;
         if (!mbar_wait(&acc_empty_bar[a], ((it >> 1) & 1) ^ 1u, p.err,
@@ -535,24 +576,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d = tmem + a * TN;
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, p.err, kErrMma)) {
+          if (!ready &&
+              !mbar_wait(&full_bar[stage], phase, p.err, kErrMma)) {
             ok = false;
             break;
           }
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          ready = mbar_peek(&full_bar[next], next_phase);
           tc_fence_after();
           const uint32_t soff =
               static_cast<uint32_t>(stage) * (Cf::kStageBytes >> 4);
           const uint32_t sf_t = tmem + Cf::kSfBase + stage * kSfCols;
           const int steps = min(4, kblk64 - 4 * kb);
-          for (int j = 0; j < steps; ++j)
-            tc_mma_nvf4(d, w_desc0 + soff + 2u * j, x_desc0 + soff + 2u * j,
-                        kIdesc, sf_t + 4 * j, sf_t + 16 + 4 * j,
-                        (kb > kb0 || j > 0) ? 1u : 0u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < steps)
+              tc_mma_nvf4(d, w_desc0 + soff + 2u * j, x_desc0 + soff + 2u * j,
+                          kIdesc, sf_t + 4 * j, sf_t + 16 + 4 * j,
+                          (kb > kb0 || j > 0) ? 1u : 0u);
           tc_commit(&empty_bar[stage]);
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
         if (ok) tc_commit(&acc_full_bar[a]);
       }
@@ -933,7 +978,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       long long issued = 0;
-      bool ok = true;
+      bool ok = true, ready = false;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
         const PairTile t = locate_pair(p, tab, tile);
@@ -950,12 +995,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                              (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
                                  kAtomBytes;
         for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (issued >= S &&
+          if (issued >= S && !ready &&
               !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
                                  kErrProducer)) {
             ok = false;
             break;
           }
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          ready = mbar_peek(&empty_bar[next], next_phase ^ 1u);
           uint8_t* st = smem + stage * kPairStageBytes;
           uint8_t* sf = st + 2 * kPairTile;
           const size_t run =
@@ -977,10 +1025,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                              row, t.g, pol);
           }
           ++issued;
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
       }
       // never leave with copies in flight: scale runs land on this CTA's
@@ -1002,15 +1048,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + ((32u * q) << 16);
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true;
+    bool ok = true, ready = false;
     griddep_wait();
     for (int tile = first; ok && tile < total; tile += step) {
       for (int kb = 0; kb < p.kblocks; ++kb) {
-        const bool got = mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
-        if (!__all_sync(0xffffffffu, got)) {
-          ok = false;
-          break;
+        if (!__all_sync(0xffffffffu, ready)) {
+          const bool got =
+              mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
+          if (!__all_sync(0xffffffffu, got)) {
+            ok = false;
+            break;
+          }
         }
+        const int next = stage + 1 == S ? 0 : stage + 1;
+        const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+        ready = mbar_peek(&sfdata_bar[next], next_phase);
         // arm the stage's next fill: it cannot complete before all four
         // scale warps have passed this one
         if (warp == kSfWarp0 && lane == 0)
@@ -1054,10 +1106,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           else
             mbar_arrive_cluster(full_s);
         }
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
-        }
+        stage = next;
+        phase = next_phase;
       }
     }
   } else if (warp == kMmaWarp) {
@@ -1070,7 +1120,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                          SmemLayout::kSwizzle128B);
       int stage = 0;
       uint32_t phase = 0, acc_phase = 0;
-      bool ok = true, any = false;
+      bool ok = true, any = false, ready = false;
       for (int tile = first; ok && tile < total; tile += step) {
         if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
                                kErrMma)) {
@@ -1079,10 +1129,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
+          if (!ready &&
+              !mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
             ok = false;
             break;
           }
+          const int next = stage + 1 == S ? 0 : stage + 1;
+          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+          ready = mbar_peek(&full_bar[next], next_phase);
           tc_fence_after();
           const uint32_t soff =
               static_cast<uint32_t>(stage) * (kPairStageBytes >> 4);
@@ -1102,10 +1156,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 0));
           any = true;
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          stage = next;
+          phase = next_phase;
         }
         if (!ok) break;
         tc_commit_pair(mapa_shared(smem_u32(&acc_full_bar), 0));
