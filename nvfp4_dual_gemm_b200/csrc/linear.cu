@@ -21,6 +21,7 @@
 #include <atomic>
 #include <cstring>
 #include <string>
+#include <type_traits>
 
 #include "host.h"
 #include "nvfp4_dual_gemm.h"
@@ -267,15 +268,26 @@ __device__ __forceinline__ float load_bias(const LinearParams& p, int g,
                     : to_f32<T>(static_cast<const T*>(p.bias)[i]);
 }
 
-// Residual of NC rows of C from row x (valid: `nv` of them), feature n.
+// Residual of NC rows of C from row x (valid: `nv` of them), feature n.  Rows
+// are addressed by 32-bit offsets from the first one, which is the same for
+// the whole warp.
 template <typename T, int NC>
 __device__ __forceinline__ void load_residual(const LinearParams& p, int x,
                                               int n, int nv, T (&r)[NC]) {
   if (p.residual == nullptr) return;
-  const T* src = static_cast<const T*>(p.residual) + (size_t)x * p.ldr + n;
+  const char* src = static_cast<const char*>(p.residual) +
+                    (size_t)x * p.ldr * sizeof(T);
+  uint32_t off = n * sizeof(T);
+  const uint32_t step = p.ldr * sizeof(T);
+  if (nv >= NC) {
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
-    if (i < nv) r[i] = src[(size_t)i * p.ldr];
+    for (int i = 0; i < NC; ++i, off += step)
+      r[i] = *reinterpret_cast<const T*>(src + off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NC; ++i, off += step)
+      if (i < nv) r[i] = *reinterpret_cast<const T*>(src + off);
+  }
 }
 
 // Epilogue of NC rows (tokens) of one feature: the accumulators v to C.
@@ -295,10 +307,18 @@ __device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
 #pragma unroll
     for (int i = 0; i < NC; ++i) v[i] += to_f32<T>(r[i]);
   }
-  T* dst = static_cast<T*>(p.C) + (size_t)x * p.ldc + n;
+  char* dst = static_cast<char*>(p.C) + (size_t)x * p.ldc * sizeof(T);
+  uint32_t off = n * sizeof(T);
+  const uint32_t step = p.ldc * sizeof(T);
+  if (nv >= NC) {
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
-    if (i < nv) dst[(size_t)i * p.ldc] = from_f32<T>(v[i]);
+    for (int i = 0; i < NC; ++i, off += step)
+      *reinterpret_cast<T*>(dst + off) = from_f32<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NC; ++i, off += step)
+      if (i < nv) *reinterpret_cast<T*>(dst + off) = from_f32<T>(v[i]);
+  }
 }
 
 template <int TN>
@@ -690,36 +710,61 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      bool landed = false;
+      // this rank's share: 32 columns at a time where it holds more than two
+      // groups (one TMEM round trip and one set of residual loads for eight
+      // groups), else group by group
+      auto share = [&](auto width) {
+        constexpr int kG = decltype(width)::value;
+        bool landed = false;
 #pragma unroll 1
-      for (int o = 0; o < n_own; ++o) {
-        const int col = 4 * (g_own + o);
-        const int rows = n < p.N ? nv - col : 0;
-        T r[4];
-        float own[4], v[4] = {0.f, 0.f, 0.f, 0.f};
-        load_residual<T, 4>(p, t.x0 + col, n, rows, r);
-        __syncwarp();
-        tc_ld_4cols(t_row + col, own);
-        tc_wait_ld();
-        if (!landed) {
-          const bool in = mbar_wait(&recv_bar, 0, p.err, kErrEpilogue);
-          if (!__all_sync(0xffffffffu, in)) break;
-          landed = true;
-        }
-        for (int s = 0; s < p.split; ++s) {
-          if (s == rank) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] += own[i];
+        for (int o = 0; o < n_own; o += kG) {
+          const int col = 4 * (g_own + o);
+          const int rows =
+              n < p.N ? min(nv - col, 4 * min(kG, n_own - o)) : 0;
+          T r[4 * kG];
+          float own[4 * kG], v[4 * kG];
+          load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
+          __syncwarp();
+          if constexpr (kG == 8) {
+            tc_ld_32cols(t_row + col, own);
+            tc_wait_ld();
+            tie32(own);
           } else {
-            const uint4 u = lds128(recv + ((s * gpr + o) * 128u + row) * 16u);
-            v[0] += __uint_as_float(u.x);
-            v[1] += __uint_as_float(u.y);
-            v[2] += __uint_as_float(u.z);
-            v[3] += __uint_as_float(u.w);
+            tc_ld_4cols(t_row + col, own);
+            tc_wait_ld();
           }
+          if (!landed) {
+            const bool in = mbar_wait(&recv_bar, 0, p.err, kErrEpilogue);
+            if (!__all_sync(0xffffffffu, in)) break;
+            landed = true;
+          }
+#pragma unroll
+          for (int i = 0; i < 4 * kG; ++i) v[i] = 0.f;
+          for (int s = 0; s < p.split; ++s) {
+            if (s == rank) {
+#pragma unroll
+              for (int i = 0; i < 4 * kG; ++i) v[i] += own[i];
+            } else {
+#pragma unroll
+              for (int q = 0; q < kG; ++q) {
+                if (o + q < n_own) {
+                  const uint4 u =
+                      lds128(recv + ((s * gpr + o + q) * 128u + row) * 16u);
+                  v[4 * q + 0] += __uint_as_float(u.x);
+                  v[4 * q + 1] += __uint_as_float(u.y);
+                  v[4 * q + 2] += __uint_as_float(u.z);
+                  v[4 * q + 3] += __uint_as_float(u.w);
+                }
+              }
+            }
+          }
+          finish<T, 4 * kG>(p, t.x0 + col, n, rows, bias, r, v);
         }
-        finish<T, 4>(p, t.x0 + col, n, rows, bias, r, v);
-      }
+      };
+      if (n_own > 2)
+        share(std::integral_constant<int, 8>());
+      else
+        share(std::integral_constant<int, 1>());
     }
   }
 
@@ -1449,6 +1494,8 @@ int check_linear(const nvfp4_linear_args* a, int groups,
       a->M > (1 << 30) || a->N > (1 << 30) || a->K > (1 << 30))
     return host_fail(NVFP4DG_ERR_INVALID, "too many tiles (M * N too large)");
   if (a->C == nullptr) return host_fail(NVFP4DG_ERR_INVALID, "C is NULL");
+  if (a->ldc >= (1 << 23) || (a->residual != nullptr && a->ldr >= (1 << 23)))
+    return host_fail(NVFP4DG_ERR_INVALID, "row pitch too large");
   if (a->ldc < a->N || (a->residual != nullptr && a->ldr < a->N))
     return host_fail(NVFP4DG_ERR_INVALID,
                      "the row pitch of C and residual must be at least N");
@@ -1516,8 +1563,10 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
     }
     if (mt[0] == 0) return NVFP4DG_OK;
   } else {
-    // counts on the device: A's rows spread evenly
-    const long long per = groups ? (a->M + groups - 1) / groups : a->M;
+    // counts on the device: A's rows spread evenly, half a row block of each
+    // group taken for padding
+    long long per = groups ? (a->M + groups - 1) / groups : a->M;
+    if (groups) per = std::max(per - 64, (per + 1) / 2);
     const long long g = groups ? groups : 1;
     mt[0] = (per + 31) / 32 * g;
     mt[1] = (per + 63) / 64 * g;
