@@ -34,13 +34,14 @@ constexpr int kFeat = 128;          // features (rows of B) per tile
 constexpr int kRowBytes = 128;      // a stage holds 256 fp4 of K per row
 constexpr int kAtomBytes = 512;     // scales of 128 rows x 64 K elements
 constexpr int kRunBytes = 4 * kAtomBytes;
-constexpr int kThreads = 352;
-constexpr int kEpiWarps = 4;
+constexpr int kThreads = 480;
+constexpr int kEpiWarps = 8;        // warps 0-3 and 11-14, see epi_group
 constexpr int kProdWWarp = 4;       // copies weights and their scales
 constexpr int kProdXWarp = 5;       // copies tokens and their scales
 constexpr int kMmaWarp = 6;
 constexpr int kSfWarp0 = 7;         // four warps, one per TMEM sub-partition
 constexpr int kSfWarps = 4;
+constexpr int kEpiWarp1 = 11;
 constexpr int kTmemCols = 512;
 constexpr int kMaxStages = 8;
 constexpr int kSfCols = 32;         // TMEM columns of a stage's scales
@@ -210,6 +211,29 @@ __device__ __forceinline__ void tc_ld_4cols(uint32_t taddr, float (&v)[4]) {
       : "memory");
 }
 
+// The epilogue warps form two groups of four that share a tile's columns: warp
+// w of a group owns TMEM lanes 32 (w % 4) .. + 31.  One group of four took
+// longer for a tile of short K than the products of the next one.
+__device__ __forceinline__ int epi_group(int warp) {
+  return warp >= kEpiWarp1 ? 1 : 0;
+}
+// Barrier of one group, and one that also ANDs a predicate.
+__device__ __forceinline__ void epi_bar(int group) {
+  asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+}
+__device__ __forceinline__ bool epi_all(int group, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(out)
+      : "r"(static_cast<uint32_t>(pred)), "r"(group + 1)
+      : "memory");
+  return out != 0;
+}
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -231,7 +255,49 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// act(v), NC values, in fp32.  silu(x) = x / (1 + e^-x);
+// x / (1 + 2^t) for two values, t clamped at 126 so that the denominator d
+// stays finite (the quotient is then below every 16-bit type's range).  The
+// reciprocal runs on the FMA pipe, two values an instruction: three Newton
+// steps r <- r + r (1 - d r) from a first guess read off the bits of d (the
+// integer 0x7EF311C3 - bits(d) is 1 / d within 11 %, and the error squares at
+// each step), which leaves one special-function operation a value: those
+// retire 16 a cycle and bounded the epilogue at two.
+__device__ __forceinline__ void quotient2(float& x0, float& x1, float t0,
+                                          float t1) {
+  asm("{\n\t"
+      ".reg .b64 X, ND, R, E, ONE;\n\t"
+      ".reg .b32 a0, a1, n0, n1, r0, r1;\n\t"
+      "mov.b64 ONE, {0x3F800000, 0x3F800000};\n\t"
+      "min.f32 a0, %2, 0f42FC0000;\n\t"  // 126
+      "min.f32 a1, %3, 0f42FC0000;\n\t"
+      "ex2.approx.ftz.f32 a0, a0;\n\t"
+      "ex2.approx.ftz.f32 a1, a1;\n\t"
+      "sub.rn.f32 n0, 0fBF800000, a0;\n\t"  // -d
+      "sub.rn.f32 n1, 0fBF800000, a1;\n\t"
+      "sub.u32 r0, 0xFEF311C3, n0;\n\t"
+      "sub.u32 r1, 0xFEF311C3, n1;\n\t"
+      "mov.b64 ND, {n0, n1};\n\t"
+      "mov.b64 R, {r0, r1};\n\t"
+      "mov.b64 X, {%0, %1};\n\t"
+      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
+      "fma.rn.f32x2 R, R, E, R;\n\t"
+      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
+      "fma.rn.f32x2 R, R, E, R;\n\t"
+      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
+      "fma.rn.f32x2 R, R, E, R;\n\t"
+      "mul.rn.f32x2 X, X, R;\n\t"
+      "mov.b64 {%0, %1}, X;\n\t"
+      "}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(t0), "f"(t1));
+}
+
+// Not inlined: 32 copies of erfc would cost the epilogue its registers.
+__device__ __noinline__ float gelu_erf(float x) {
+  return 0.5f * x * erfcf(-0.7071067811865476f * x);
+}
+
+// act(v), NC values (an even number), in fp32.  silu(x) = x / (1 + e^-x);
 // 0.5 (1 + tanh u) = 1 / (1 + e^-2u), so the tanh form of gelu is
 // x / (1 + e^-2u) with u = sqrt(2/pi) (x + 0.044715 x^3); the erf form is
 // 0.5 x erfc(-x / sqrt 2), which keeps its digits for negative x.
@@ -242,20 +308,21 @@ __device__ __forceinline__ void activate(float (&v)[NC], int act) {
 #pragma unroll
     for (int i = 0; i < NC; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // keeps NaN
   } else if (act == NVFP4DG_ACT_SILU) {
+    constexpr float k = -1.4426950408889634f;  // -log2(e)
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      v[i] = __fdividef(v[i], 1.f + __expf(-v[i]));
+    for (int i = 0; i < NC; i += 2)
+      quotient2(v[i], v[i + 1], k * v[i], k * v[i + 1]);
   } else if (act == NVFP4DG_ACT_GELU_TANH) {
+    constexpr float k = -2.302208198201456f;  // -2 sqrt(2/pi) log2(e)
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const float x = v[i];
-      const float m2u = -1.5957691216057308f * x * fmaf(0.044715f, x * x, 1.f);
-      v[i] = __fdividef(x, 1.f + __expf(m2u));
+    for (int i = 0; i < NC; i += 2) {
+      const float x = v[i], y = v[i + 1];
+      quotient2(v[i], v[i + 1], k * x * fmaf(0.044715f, x * x, 1.f),
+                k * y * fmaf(0.044715f, y * y, 1.f));
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      v[i] = 0.5f * v[i] * erfcf(-0.7071067811865476f * v[i]);
+    for (int i = 0; i < NC; ++i) v[i] = gelu_erf(v[i]);
   }
 }
 
@@ -499,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= kSfWarp0) {
+  } else if (warp >= kSfWarp0 && warp < kEpiWarp1) {
     // ---------------------------------------------------------- scale warps
     // Lane 32q + i, column c of a K step's four columns holds the scales of
     // rows i + 32c of the 128-row block.  A tile of TN < 128 tokens starts
@@ -628,22 +695,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (p.split == 1) {
     // ---------------------------------------------------------- epilogue
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int q = warp % 4, group = epi_group(warp);
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16);
     int it = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, ++it) {
       const Tile t = locate<TN>(p, tab, tile);
       const int a = it & 1;
-      const int n = t.n0 + threadIdx.x;
+      const int n = t.n0 + 32 * q + lane;
       const float bias = load_bias<T>(p, t.g, n);
-      const int rows = n < p.N ? min(t.rows, TN) : 0;
+      const int cols = min(t.rows, TN);
+      const int rows = n < p.N ? cols : 0;
       const bool got =
           mbar_wait(&acc_full_bar[a], (it >> 1) & 1, p.err, kErrEpilogue);
       if (!__all_sync(0xffffffffu, got)) break;
       tc_fence_after();
-      const int last = (min(t.rows, TN) - 1) / 32;
+      // the groups take chunks of 32 columns in turn
 #pragma unroll 1
-      for (int c = 0; c <= last; ++c) {
+      for (int c = group; 32 * c < cols; c += 2) {
         T r[32];
         float v[32];
         load_residual<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, r);
@@ -651,21 +720,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_ld_32cols(t_row + a * TN + 32 * c, v);
         tc_wait_ld();
         tie32(v);
-        if (c == last) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&acc_empty_bar[a]);
-        }
         finish<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, bias, r, v);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty_bar[a]);
     }
   } else {
     // ---------------------------------------------------------- split-K
-    // Groups of four token columns; rank d finishes groups
-    // [d * gpr, (d + 1) * gpr).  In the receive buffer, source s, own group
+    // Pieces of four token columns; rank d finishes pieces
+    // [d * gpr, (d + 1) * gpr).  In the receive buffer, source s, own piece
     // j, row r sit at ((s * gpr + j) * 128 + r) * 16.
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const int row = threadIdx.x;
+    const int q4 = warp % 4, group = epi_group(warp);
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
+    const int row = 32 * q4 + lane;
     const Tile t = locate<TN>(p, tab, first);
     const int nv = min(t.rows, TN);
     const int g4 = (nv + 3) / 4;
@@ -681,56 +749,57 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool got = mbar_wait(&acc_full_bar[0], 0, p.err, kErrEpilogue);
     if (__all_sync(0xffffffffu, got)) {
       tc_fence_after();
-      int d = 0, j = 0;  // rank and its group
-      uint32_t dst = 0, bar = 0;
 #pragma unroll 1
-      for (int c = 0; 8 * c < g4; ++c) {
+      for (int c = group; 8 * c < g4; c += 2) {
         float v[32];
         __syncwarp();
         tc_ld_32cols(t_row + 32 * c, v);
         tc_wait_ld();
         tie32(v);
+        int d = 8 * c / gpr;       // rank of the piece
+        int j = 8 * c - d * gpr;   // its number there
+        uint32_t dst = mapa_shared(recv, d);
+        uint32_t bar = mapa_shared(smem_u32(&recv_bar), d);
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           if (8 * c + q < g4) {
-            if (j == 0) {
-              dst = mapa_shared(recv, d);
-              bar = mapa_shared(smem_u32(&recv_bar), d);
-            }
             if (d != rank) {
               const float f[4] = {v[4 * q], v[4 * q + 1], v[4 * q + 2],
                                   v[4 * q + 3]};
               st_async_v4(dst + ((rank * gpr + j) * 128u + row) * 16u, f,
                           bar);
             }
-            if (++j == gpr) {
+            if (++j == gpr && 8 * c + q + 1 < g4) {
               j = 0;
               ++d;
+              dst = mapa_shared(recv, d);
+              bar = mapa_shared(smem_u32(&recv_bar), d);
             }
           }
         }
       }
       // this rank's share: 32 columns at a time where it holds more than two
-      // groups (one TMEM round trip and one set of residual loads for eight
-      // groups), else group by group
+      // pieces (one TMEM round trip and one set of residual loads for eight),
+      // else piece by piece; the groups of warps take them in turn.  Partials
+      // are added in rank order after the rank's own.
       auto share = [&](auto width) {
         constexpr int kG = decltype(width)::value;
         bool landed = false;
 #pragma unroll 1
-        for (int o = 0; o < n_own; o += kG) {
+        for (int o = group * kG; o < n_own; o += 2 * kG) {
           const int col = 4 * (g_own + o);
           const int rows =
               n < p.N ? min(nv - col, 4 * min(kG, n_own - o)) : 0;
           T r[4 * kG];
-          float own[4 * kG], v[4 * kG];
+          float v[4 * kG];
           load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
           __syncwarp();
           if constexpr (kG == 8) {
-            tc_ld_32cols(t_row + col, own);
+            tc_ld_32cols(t_row + col, v);
             tc_wait_ld();
-            tie32(own);
+            tie32(v);
           } else {
-            tc_ld_4cols(t_row + col, own);
+            tc_ld_4cols(t_row + col, v);
             tc_wait_ld();
           }
           if (!landed) {
@@ -738,23 +807,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!__all_sync(0xffffffffu, in)) break;
             landed = true;
           }
-#pragma unroll
-          for (int i = 0; i < 4 * kG; ++i) v[i] = 0.f;
           for (int s = 0; s < p.split; ++s) {
-            if (s == rank) {
+            if (s == rank) continue;
 #pragma unroll
-              for (int i = 0; i < 4 * kG; ++i) v[i] += own[i];
-            } else {
-#pragma unroll
-              for (int q = 0; q < kG; ++q) {
-                if (o + q < n_own) {
-                  const uint4 u =
-                      lds128(recv + ((s * gpr + o + q) * 128u + row) * 16u);
-                  v[4 * q + 0] += __uint_as_float(u.x);
-                  v[4 * q + 1] += __uint_as_float(u.y);
-                  v[4 * q + 2] += __uint_as_float(u.z);
-                  v[4 * q + 3] += __uint_as_float(u.w);
-                }
+            for (int q = 0; q < kG; ++q) {
+              if (o + q < n_own) {
+                const uint4 u =
+                    lds128(recv + ((s * gpr + o + q) * 128u + row) * 16u);
+                v[4 * q + 0] += __uint_as_float(u.x);
+                v[4 * q + 1] += __uint_as_float(u.y);
+                v[4 * q + 2] += __uint_as_float(u.z);
+                v[4 * q + 3] += __uint_as_float(u.w);
               }
             }
           }
@@ -844,23 +907,6 @@ __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
   t.rows = rows - m0;
   t.sfa_last = (tab.row0[lo] + rows - 1) / 128;
   return t;
-}
-
-// Barrier of the four epilogue warps, and one that also ANDs a predicate.
-__device__ __forceinline__ void epi_bar() {
-  asm volatile("bar.sync 1, 128;" ::: "memory");
-}
-__device__ __forceinline__ bool epi_all(bool pred) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, 1, 128, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(out)
-      : "r"(static_cast<uint32_t>(pred))
-      : "memory");
-  return out != 0;
 }
 
 template <typename T>
@@ -1087,7 +1133,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= kSfWarp0) {
+  } else if (warp >= kSfWarp0 && warp < kEpiWarp1) {
     // ---------------------------------------------------------- scale warps
     const uint32_t q = static_cast<uint32_t>(warp % 4);
     const uint32_t t_lane = tmem + ((32u * q) << 16);
@@ -1220,12 +1266,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ---------------------------------------------------------- epilogue
-    const int row = threadIdx.x;
-    const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    // Each group of four warps finishes 128 of the tile's columns in two
+    // phases of 64, through a box of its own.
+    const int q4 = warp % 4, group = epi_group(warp);
+    const int row = 32 * q4 + lane;
+    const bool stores = row == 0;  // the thread that stores the group's box
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const uint32_t acc_empty_c = mapa_shared(smem_u32(&acc_empty_bar), 0);
-    uint8_t* boxes = smem + S * kPairStageBytes;
+    uint8_t* box = smem + S * kPairStageBytes + group * kBoxBytes;
+    float* bias = bias_sh + 128 * group;
     uint32_t acc_phase = 0;
-    int stores = 0;  // boxes stored, alternately
     griddep_wait();
     for (int tile = first; tile < total; tile += step, acc_phase ^= 1u) {
       const PairTile t = locate_pair(p, tab, tile);
@@ -1234,45 +1284,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = row < rows;
       const float scale =
           p.row_scale != nullptr && live ? p.row_scale[x] : 0.f;
-      epi_bar();  // the previous tile's bias has been read
-      bias_sh[row] = load_bias<T>(p, t.g, t.n0 + row);
-      bias_sh[row + 128] = load_bias<T>(p, t.g, t.n0 + row + 128);
+      const int n0 = t.n0 + 128 * group;
+      epi_bar(group);  // the previous tile's bias has been read
+      bias[row] = load_bias<T>(p, t.g, n0 + row);
       const bool got =
           mbar_wait_cluster(&acc_full_bar, acc_phase, p.err, kErrEpilogue);
       // the four warps leave together: they meet at the barriers below
-      if (!epi_all(got)) break;
+      if (!epi_all(group, got)) break;
       tc_fence_after();
       // a group's last rows are stored row by row: a box would overwrite the
       // rows behind them
       const bool boxed = p.groups == 0 ? rows > 0 : rows >= 128;
 #pragma unroll 1
-      for (int ph = 0; ph < 4; ++ph) {
+      for (int ph = 0; ph < 2; ++ph) {
+        const int n = n0 + 64 * ph;
         float v[2][32];
         __syncwarp();
-        tc_ld_32cols(t_row + 64 * ph, v[0]);
-        tc_ld_32cols(t_row + 64 * ph + 32, v[1]);
+        tc_ld_32cols(t_row + 128 * group + 64 * ph, v[0]);
+        tc_ld_32cols(t_row + 128 * group + 64 * ph + 32, v[1]);
         tc_wait_ld();
         tie32(v[0]);
         tie32(v[1]);
-        if (ph == 3) {
+        if (ph == 1) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc_empty_c);
         }
-        const int n = t.n0 + 64 * ph;
         if (n >= p.N) continue;
-        uint8_t* box = boxes + (stores & 1) * kBoxBytes;
         if (boxed) {
-          // the store before last read this box
-          if (threadIdx.x == 0)
-            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          epi_bar();
+          // the store before has read the box
+          if (stores) bulk_wait_group_read0();
+          epi_bar(group);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 o[4];
           finish_row32<T>(p, x, n + 32 * h, live, scale,
-                          bias_sh + 64 * ph + 32 * h, v[h], o);
+                          bias + 64 * ph + 32 * h, v[h], o);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             if (boxed)
@@ -1287,17 +1335,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (boxed) {
           fence_proxy_async_smem();
-          epi_bar();
-          if (threadIdx.x == 0) {
-            tma_store_2d(&tmC, box, 2 * n, t.x0 + 128 * static_cast<int>(rank));
+          epi_bar(group);
+          if (stores) {
+            tma_store_2d(&tmC, box, 2 * n,
+                         t.x0 + 128 * static_cast<int>(rank));
             bulk_commit_group();
           }
-          ++stores;
         }
       }
     }
     // the stores must have read their boxes before shared memory goes away
-    if (threadIdx.x == 0) bulk_wait_group_read0();
+    if (stores) bulk_wait_group_read0();
     __syncwarp();
   }
 
