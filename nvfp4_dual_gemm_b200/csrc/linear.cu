@@ -44,14 +44,13 @@ constexpr int kSfWarps = 4;
 constexpr int kEpiWarp1 = 11;
 constexpr int kTmemCols = 512;
 constexpr int kMaxStages = 8;
-constexpr int kSfCols = 32;         // TMEM columns of a stage's scales
 constexpr int kMaxSplit = 8;
 constexpr int kMaxGroups = 256;
 constexpr int kSmemBudget = 221 * 1024;  // dynamic; static holds the groups
 
 struct LinearParams {
   int M, N, K;       // M: rows of A and C (of all groups)
-  int kblocks;       // ceil(K / 256)
+  int kblocks;       // K blocks of a tile (the kernel's block: 256 or 512)
   int n_tiles;       // ceil(N / 128)
   int m_tiles;       // ceil(M / TN) (one problem)
   int split;         // CTAs of a cluster that share a tile's K range
@@ -388,11 +387,22 @@ __device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
   }
 }
 
+// A stage of linear_kernel's ring holds kSub blocks of 256 along K.  What a
+// stage costs beyond its bytes, a wait of ~300 cycles in each role and the MMA
+// thread's commit, made a 256-wide block take ~710 cycles; two of them at once
+// take less than twice the half (460 each).  With 128 tokens a stage is twice
+// as deep in bytes and one block wide.
 template <int TN>
 struct Cfg {
-  static constexpr int kWBytes = kFeat * kRowBytes;
-  static constexpr int kXBytes = TN * kRowBytes;
-  static constexpr int kStageBytes = kWBytes + kXBytes + 2 * kRunBytes;
+  static constexpr int kSub = TN <= 64 ? 2 : 1;
+  static constexpr int kSteps = 4 * kSub;  // MMAs of 64 along K
+  static constexpr int kWBox = kFeat * kRowBytes;
+  static constexpr int kXBox = TN * kRowBytes;
+  static constexpr int kWBytes = kSub * kWBox;
+  static constexpr int kXBytes = kSub * kXBox;
+  static constexpr int kRun = kSub * kRunBytes;
+  static constexpr int kSfCols = 32 * kSub;  // TMEM columns of its scales
+  static constexpr int kStageBytes = kWBytes + kXBytes + 2 * kRun;
   // split-K: the partials a CTA receives, fp32
   static constexpr int kRecvBytes = kFeat * TN * 4;
   static constexpr int kSfBase = 2 * TN;  // two accumulators, then scales
@@ -409,11 +419,11 @@ struct Cfg {
   static_assert(kStageBytes % 1024 == 0, "stages stay 1024-byte aligned");
 };
 
-// Per 256-wide K block the two producer warps copy a [128 x 128 B] weight
-// tile, a [TN x 128 B] token tile and their scale runs into a ring stage;
-// four scale warps move the scales into TMEM; one thread issues four
-// block-scaled MMAs (M = 128 features, N = TN tokens, K = 64) and four warps
-// finish the tile.  Two accumulators, so that a tile's epilogue runs under
+// Per K block the two producer warps copy [128 x 128 B] boxes of weights, [TN x
+// 128 B] boxes of tokens and their scale runs into a ring stage; four scale
+// warps move the scales into TMEM; one thread issues a block-scaled MMA
+// (M = 128 features, N = TN tokens) for each 64 of K and eight warps finish
+// the tile.  Two accumulators, so that a tile's epilogue runs under
 // the next tile's products.  K needs only be a multiple of 64: the last
 // block's missing 64-wide steps are not issued.
 //
@@ -445,10 +455,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int kblk64 = p.K / 64;
   // A K block's scale run has the same size for every block: the last
-  // block's, when K % 256 != 0, starts earlier and its first atoms are
+  // block's, when it is short, starts earlier and its first atoms are
   // skipped (`skip` in the scale warps).
   const uint32_t run_bytes =
-      static_cast<uint32_t>(min(4, kblk64)) * kAtomBytes;
+      static_cast<uint32_t>(min(Cf::kSteps, kblk64)) * kAtomBytes;
 
   if (warp == 0) {
     uint64_t* bar = nullptr;
@@ -520,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t pol = w_side ? kPolicyEvictNormal : kPolicyEvictLast;
       const uint32_t tile_off = w_side ? 0 : Cf::kWBytes;
       const uint32_t sf_off =
-          Cf::kWBytes + Cf::kXBytes + (w_side ? 0 : kRunBytes);
+          Cf::kWBytes + Cf::kXBytes + (w_side ? 0 : Cf::kRun);
       int stage = 0;
       uint32_t phase = 0;
       long long issued = 0;
@@ -546,10 +556,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           ready = mbar_peek(&empty_bar[next], next_phase ^ 1u);
           uint8_t* st = smem + stage * Cf::kStageBytes;
           bulk_load(st + sf_off,
-                    sf + (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes,
+                    sf + (size_t)min(Cf::kSteps * kb,
+                                     max(0, kblk64 - Cf::kSteps)) *
+                             kAtomBytes,
                     run_bytes, &sfdata_bar[stage], pol);
-          tma_load_3d(st + tile_off, tm, &full_bar[stage], kb * kRowBytes,
-                      row, layer, pol);
+#pragma unroll
+          for (int h = 0; h < Cf::kSub; ++h)  // (zeros beyond K)
+            tma_load_3d(st + tile_off + h * (w_side ? Cf::kWBox : Cf::kXBox),
+                        tm, &full_bar[stage],
+                        (kb * Cf::kSub + h) * kRowBytes, row, layer, pol);
           ++issued;
           stage = next;
           phase = next_phase;
@@ -596,37 +611,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         // scale warps have passed this one
         if (warp == kSfWarp0 && lane == 0)
           mbar_arrive_expect_tx(&sfdata_bar[stage], 2 * run_bytes);
-        const int skip = 4 * kb - min(4 * kb, max(0, kblk64 - 4));
+        const int skip =
+            Cf::kSteps * kb -
+            min(Cf::kSteps * kb, max(0, kblk64 - Cf::kSteps));
         const uint32_t sf_s = smem_u32(smem + stage * Cf::kStageBytes +
                                        Cf::kWBytes + Cf::kXBytes) +
                               16u * lane;
-        uint32_t r[32];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // (past the run for the steps of a short block that are not issued)
-          const uint32_t at = sf_s + min(j + skip, 3) * kAtomBytes;
-          const uint4 w = lds128(at);
-          const uint4 x = lds128(at + kRunBytes);
-          r[4 * j + 0] = w.x;
-          r[4 * j + 1] = w.y;
-          r[4 * j + 2] = w.z;
-          r[4 * j + 3] = w.w;
-          if (TN == 128) {
-            r[16 + 4 * j + 0] = x.x;
-            r[16 + 4 * j + 1] = x.y;
-          } else if (TN == 64) {
-            r[16 + 4 * j + 0] = part ? x.z : x.x;
-            r[16 + 4 * j + 1] = part ? x.w : x.y;
-          } else {
-            r[16 + 4 * j + 0] =
-                part < 2 ? (part ? x.y : x.x) : (part == 2 ? x.z : x.w);
-            r[16 + 4 * j + 1] = x.y;
+        for (int h = 0; h < Cf::kSub; ++h) {
+          uint32_t r[32];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            // (past the run for the steps of a short block that are not
+            // issued)
+            const uint32_t at =
+                sf_s + min(4 * h + j + skip, Cf::kSteps - 1) * kAtomBytes;
+            const uint4 w = lds128(at);
+            const uint4 x = lds128(at + Cf::kRun);
+            r[4 * j + 0] = w.x;
+            r[4 * j + 1] = w.y;
+            r[4 * j + 2] = w.z;
+            r[4 * j + 3] = w.w;
+            if (TN == 128) {
+              r[16 + 4 * j + 0] = x.x;
+              r[16 + 4 * j + 1] = x.y;
+            } else if (TN == 64) {
+              r[16 + 4 * j + 0] = part ? x.z : x.x;
+              r[16 + 4 * j + 1] = part ? x.w : x.y;
+            } else {
+              r[16 + 4 * j + 0] =
+                  part < 2 ? (part ? x.y : x.x) : (part == 2 ? x.z : x.w);
+              r[16 + 4 * j + 1] = x.y;
+            }
+            r[16 + 4 * j + 2] = x.z;
+            r[16 + 4 * j + 3] = x.w;
           }
-          r[16 + 4 * j + 2] = x.z;
-          r[16 + 4 * j + 3] = x.w;
+          __syncwarp();
+          tc_st_32cols(t_lane + Cf::kSfBase + stage * Cf::kSfCols + 32 * h,
+                       r);
         }
-        __syncwarp();
-        tc_st_32cols(t_lane + Cf::kSfBase + stage * kSfCols, r);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -674,14 +697,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint32_t soff =
               static_cast<uint32_t>(stage) * (Cf::kStageBytes >> 4);
-          const uint32_t sf_t = tmem + Cf::kSfBase + stage * kSfCols;
-          const int steps = min(4, kblk64 - 4 * kb);
+          const uint32_t sf_t = tmem + Cf::kSfBase + stage * Cf::kSfCols;
+          const int steps = min(Cf::kSteps, kblk64 - Cf::kSteps * kb);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < Cf::kSteps; ++j)
             if (j < steps)
-              tc_mma_nvf4(d, w_desc0 + soff + 2u * j, x_desc0 + soff + 2u * j,
-                          kIdesc, sf_t + 4 * j, sf_t + 16 + 4 * j,
-                          (kb > kb0 || j > 0) ? 1u : 0u);
+              tc_mma_nvf4(
+                  d, w_desc0 + soff + (j / 4) * (Cf::kWBox >> 4) + 2u * (j % 4),
+                  x_desc0 + soff + (j / 4) * (Cf::kXBox >> 4) + 2u * (j % 4),
+                  kIdesc, sf_t + 32 * (j / 4) + 4 * (j % 4),
+                  sf_t + 32 * (j / 4) + 16 + 4 * (j % 4),
+                  (kb > kb0 || j > 0) ? 1u : 0u);
           tc_commit(&empty_bar[stage]);
           stage = next;
           phase = next_phase;
@@ -1367,6 +1393,7 @@ struct LinearPlan {
   int split;   // CTAs that share a tile's K range
   int grid;    // CTAs
   int tiles;
+  int kblocks;
 };
 
 // `mt`: token tiles of 32, 64, 128 and 256 tokens (of all groups).
@@ -1389,6 +1416,7 @@ LinearPlan plan_linear(const long long (&mts)[4], int N, int K, int groups,
                    (!forced_tile && mts[2] > mts[3] && pair_cost < one_cost))) {
     pl.tn = 256;
     pl.split = 1;
+    pl.kblocks = kblocks;
     pl.tiles = static_cast<int>(std::min<long long>(pair_tiles, 1 << 30));
     pl.grid = 2 * static_cast<int>(std::min<long long>(pair_tiles, units));
     return pl;
@@ -1406,18 +1434,20 @@ LinearPlan plan_linear(const long long (&mts)[4], int N, int K, int groups,
   const long long mt = pl.tn == 32 ? mts[0] : pl.tn == 64 ? mts[1] : mts[2];
   pl.tiles = static_cast<int>(std::min<long long>(mt * n_tiles, 1 << 30));
   pl.split = 1;
+  pl.kblocks = pl.tn <= 64 ? (K + 511) / 512 : kblocks;
   const int forced =
       static_cast<int>((flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8);
   if (groups == 0 && forced > 0) {
     pl.split = 1 << (forced - 1);
   } else if (groups == 0) {
     for (int s = kMaxSplit; s > 1; s /= 2)
-      if ((long long)pl.tiles * s <= sms && kblocks >= 2 * s) {
+      if ((long long)pl.tiles * s <= sms && kblocks >= 2 * s &&
+          pl.kblocks >= s) {
         pl.split = s;
         break;
       }
   }
-  pl.split = std::min(pl.split, std::max(kblocks, 1));
+  pl.split = std::min(pl.split, pl.kblocks);
   while (pl.split & (pl.split - 1)) --pl.split;
   pl.grid = pl.split > 1 ? pl.tiles * pl.split : std::min(pl.tiles, sms);
   return pl;
@@ -1630,7 +1660,7 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   p.M = a->M;
   p.N = a->N;
   p.K = a->K;
-  p.kblocks = (a->K + 255) / 256;
+  p.kblocks = pl.kblocks;
   p.n_tiles = (a->N + kFeat - 1) / kFeat;
   p.split = pl.split;
   p.sfa = static_cast<const uint8_t*>(a->SFA);
