@@ -94,6 +94,31 @@ __device__ __forceinline__ int group_rows(const LinearParams& p, int g,
   return min(max(n, 0), p.M - row0);
 }
 
+// A tile's place among the groups, found by a whole warp: each lane holds the
+// first tiles of groups lane, lane + 32, ... in registers, and the groups that
+// start at or below the tile are counted by votes.  (A search of the table in
+// shared memory by the one thread that needs it took ~1500 cycles a tile, as
+// long as a tile of short K.)
+struct GroupFinder {
+  int tile0[kMaxGroups / 32];
+  __device__ __forceinline__ void set(const LinearParams& p,
+                                      const GroupTable& tab, int lane) {
+#pragma unroll
+    for (int k = 0; k < kMaxGroups / 32; ++k)
+      tile0[k] = 32 * k + lane < p.groups ? tab.tile0[32 * k + lane]
+                                          : 0x7fffffff;
+  }
+  // the last group whose first tile is <= tile (empty groups have none)
+  __device__ __forceinline__ int find(const LinearParams& p, int tile) const {
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kMaxGroups / 32; ++k)
+      if (32 * k < p.groups)
+        n += __popc(__ballot_sync(0xffffffffu, tile0[k] <= tile));
+    return n - 1;
+  }
+};
+
 struct Tile {
   int g;       // group (batch of B)
   int n0;      // first feature
@@ -150,36 +175,30 @@ __device__ __forceinline__ void build_groups(const LinearParams& p, int tn,
 }
 
 // Token tiles fastest, so that CTAs of neighbouring tiles read the same
-// weights at the same time.
+// weights at the same time.  Called by whole warps.
 template <int TN>
 __device__ __forceinline__ Tile locate(const LinearParams& p,
-                                       const GroupTable& tab, int tile) {
+                                       const GroupTable& tab,
+                                       const GroupFinder& find, int tile) {
   Tile t;
   if (p.groups == 0) {
-    const int nt = tile / p.m_tiles;
+    const int nt = p.m_tiles == 1 ? tile : tile / p.m_tiles;
     t.g = 0;
     t.n0 = nt * kFeat;
     t.x0 = (tile - nt * p.m_tiles) * TN;
     t.rows = p.M - t.x0;
     return t;
   }
-  // the last group whose first tile is <= tile (empty groups have none)
-  int lo = 0, hi = p.groups - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.tile0[mid] <= tile)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int local = tile - tab.tile0[lo];
-  const int rows = group_rows(p, lo, tab.row0[lo]);
+  const int g = find.find(p, tile);
+  const int local = tile - tab.tile0[g];
+  const int row0 = tab.row0[g];
+  const int rows = group_rows(p, g, row0);
   const int mt = (rows + TN - 1) / TN;
-  const int nt = local / mt;
+  const int nt = mt == 1 ? local : local / mt;
   const int m0 = (local - nt * mt) * TN;
-  t.g = lo;
+  t.g = g;
   t.n0 = nt * kFeat;
-  t.x0 = tab.row0[lo] + m0;
+  t.x0 = row0 + m0;
   t.rows = rows - m0;
   return t;
 }
@@ -356,18 +375,25 @@ __device__ __forceinline__ void load_residual(const LinearParams& p, int x,
   }
 }
 
+// Row scale of row x + i for lane i (valid: `nv` rows).
+__device__ __forceinline__ float load_scale(const LinearParams& p, int x,
+                                            int nv, int lane) {
+  return p.row_scale != nullptr && lane < nv ? p.row_scale[x + lane] : 0.f;
+}
+
 // Epilogue of NC rows (tokens) of one feature: the accumulators v to C.
+// `scale`: lane i holds the row scale of row i (NC <= 32).
 template <typename T, int NC>
 __device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
-                                       int nv, float bias, const T (&r)[NC],
-                                       float (&v)[NC]) {
+                                       int nv, float bias, float scale,
+                                       const T (&r)[NC], float (&v)[NC]) {
 #pragma unroll
   for (int i = 0; i < NC; ++i) v[i] = fmaf(p.alpha, v[i], bias);
   activate<NC>(v, p.act);
   if (p.row_scale != nullptr) {
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-      if (i < nv) v[i] *= p.row_scale[x + i];
+      v[i] *= __shfl_sync(0xffffffffu, scale, i);
   }
   if (p.residual != nullptr) {
 #pragma unroll
@@ -513,6 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int total =
       p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
+  GroupFinder find;
+  if (p.groups > 0) find.set(p, tab, lane);
   const int first = static_cast<int>(blockIdx.x) / p.split;
   const int step = static_cast<int>(gridDim.x) / p.split;
   const int kb0 = static_cast<int>((long long)p.kblocks * rank / p.split);
@@ -524,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // They only copy: a thread's instructions on barriers and copies take
     // ~105 cycles each, and with the arming of both barriers in this loop a K
     // block took ~1000 cycles whatever its size.
-    if (lane == 0) {
+    {
       const bool w_side = warp == kProdWWarp;
       const CUtensorMap* tm = w_side ? &tmW : &tmX;
       const uint64_t pol = w_side ? kPolicyEvictNormal : kPolicyEvictLast;
@@ -537,14 +565,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true, ready = false;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
-        const Tile t = locate<TN>(p, tab, tile);
+        const Tile t = locate<TN>(p, tab, find, tile);  // the whole warp
         const uint8_t* sf =
             w_side ? p.sfb + (size_t)t.g * p.sfb_group +
                          (size_t)(t.n0 / 128) * kblk64 * kAtomBytes
                    : p.sfa + (size_t)(t.x0 / 128) * kblk64 * kAtomBytes;
         const int row = w_side ? t.n0 : t.x0;
         const int layer = w_side ? t.g : 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int kb = kb0; lane == 0 && kb < kb1; ++kb) {
           if (issued >= S && !ready &&
               !mbar_wait(&empty_bar[stage], phase ^ 1u, p.err,
                          kErrProducer)) {
@@ -569,9 +597,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage = next;
           phase = next_phase;
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       // never leave with copies in flight
-      for (int s = 0; s < S; ++s) {
+      for (int s = 0; s < S; ++s) {  // (lane 0 has issued all)
         if (issued > s) {
           const uint32_t par =
               static_cast<uint32_t>(((issued - 1 - s) / S) & 1);
@@ -594,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_wait();
     for (int tile = first; ok && tile < total; tile += step) {
       const int part =
-          TN == 128 ? 0 : (locate<TN>(p, tab, tile).x0 % 128) / 32;
+          TN == 128 ? 0 : (locate<TN>(p, tab, find, tile).x0 % 128) / 32;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!__all_sync(0xffffffffu, ready)) {
           const bool got =
@@ -726,12 +755,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, ++it) {
-      const Tile t = locate<TN>(p, tab, tile);
+      const Tile t = locate<TN>(p, tab, find, tile);
       const int a = it & 1;
       const int n = t.n0 + 32 * q + lane;
       const float bias = load_bias<T>(p, t.g, n);
       const int cols = min(t.rows, TN);
       const int rows = n < p.N ? cols : 0;
+      // (with the bias, before the wait: their latency passes meanwhile)
+      const float scale0 =
+          load_scale(p, t.x0 + 32 * group, cols - 32 * group, lane);
       const bool got =
           mbar_wait(&acc_full_bar[a], (it >> 1) & 1, p.err, kErrEpilogue);
       if (!__all_sync(0xffffffffu, got)) break;
@@ -742,11 +774,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         T r[32];
         float v[32];
         load_residual<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, r);
+        const float scale =
+            c == group ? scale0
+                       : load_scale(p, t.x0 + 32 * c, cols - 32 * c, lane);
         __syncwarp();
         tc_ld_32cols(t_row + a * TN + 32 * c, v);
         tc_wait_ld();
         tie32(v);
-        finish<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, bias, r, v);
+        finish<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, bias, scale, r, v);
       }
       tc_fence_before();
       __syncwarp();
@@ -760,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q4 = warp % 4, group = epi_group(warp);
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const int row = 32 * q4 + lane;
-    const Tile t = locate<TN>(p, tab, first);
+    const Tile t = locate<TN>(p, tab, find, first);
     const int nv = min(t.rows, TN);
     const int g4 = (nv + 3) / 4;
     const int gpr = (g4 + p.split - 1) / p.split;
@@ -819,6 +854,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           T r[4 * kG];
           float v[4 * kG];
           load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
+          const float scale = load_scale(
+              p, t.x0 + col, min(nv - col, 4 * min(kG, n_own - o)), lane);
           __syncwarp();
           if constexpr (kG == 8) {
             tc_ld_32cols(t_row + col, v);
@@ -847,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          finish<T, 4 * kG>(p, t.x0 + col, n, rows, bias, r, v);
+          finish<T, 4 * kG>(p, t.x0 + col, n, rows, bias, scale, r, v);
         }
       };
       if (n_own > 2)
@@ -899,6 +936,7 @@ struct PairTile {
 // operand rows than whole columns of m tiles do.
 __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
                                                 const GroupTable& tab,
+                                                const GroupFinder& find,
                                                 int tile) {
   PairTile t;
   if (p.groups == 0) {
@@ -914,24 +952,18 @@ __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
     t.sfa_last = (p.M - 1) / 128;
     return t;
   }
-  int lo = 0, hi = p.groups - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (tab.tile0[mid] <= tile)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int local = tile - tab.tile0[lo];
-  const int rows = group_rows(p, lo, tab.row0[lo]);
+  const int g = find.find(p, tile);
+  const int local = tile - tab.tile0[g];
+  const int row0 = tab.row0[g];
+  const int rows = group_rows(p, g, row0);
   const int mt = (rows + 255) / 256;
-  const int nt = local / mt;
+  const int nt = mt == 1 ? local : local / mt;
   const int m0 = (local - nt * mt) * 256;
-  t.g = lo;
+  t.g = g;
   t.n0 = nt * 256;
-  t.x0 = tab.row0[lo] + m0;
+  t.x0 = row0 + m0;
   t.rows = rows - m0;
-  t.sfa_last = (tab.row0[lo] + rows - 1) / 128;
+  t.sfa_last = (row0 + rows - 1) / 128;
   return t;
 }
 
@@ -1080,6 +1112,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base_sh;
   const int total =
       p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
+  GroupFinder find;
+  if (p.groups > 0) find.set(p, tab, lane);
   const int first = static_cast<int>(blockIdx.x) / 2;
   const int step = static_cast<int>(gridDim.x) / 2;
 
@@ -1088,7 +1122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Warp 4: token scales, the first run of weight scales, token rows; warp
     // 5: the second run, weight rows.  They only copy: the expected bytes
     // come with the scale warps' arrivals.
-    if (lane == 0) {
+    {
       const bool x_side = warp == kProdWWarp;
       const uint64_t pol = x_side ? kPolicyEvictLast : kPolicyEvictNormal;
       const uint32_t full_c = mapa_shared(smem_u32(&full_bar[0]), 0);
@@ -1098,7 +1132,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true, ready = false;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
-        const PairTile t = locate_pair(p, tab, tile);
+        const PairTile t = locate_pair(p, tab, find, tile);
         const int row = (x_side ? t.x0 : t.n0) + 128 * static_cast<int>(rank);
         // the odd CTA's rows may lie past the problem's last row block, and
         // the second weight run past the last one: they copy the last, whose
@@ -1111,7 +1145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* sfb = p.sfb + (size_t)t.g * p.sfb_group +
                              (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
                                  kAtomBytes;
-        for (int kb = 0; kb < p.kblocks; ++kb) {
+        for (int kb = 0; lane == 0 && kb < p.kblocks; ++kb) {
           if (issued >= S && !ready &&
               !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
                                  kErrProducer)) {
@@ -1145,6 +1179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           stage = next;
           phase = next_phase;
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       // never leave with copies in flight: scale runs land on this CTA's
       // barriers, both CTAs' tiles on the even one's
@@ -1304,7 +1339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_phase = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, acc_phase ^= 1u) {
-      const PairTile t = locate_pair(p, tab, tile);
+      const PairTile t = locate_pair(p, tab, find, tile);
       const int rows = t.rows - 128 * static_cast<int>(rank);  // of this CTA
       const int x = t.x0 + 128 * static_cast<int>(rank) + row;
       const bool live = row < rows;
