@@ -273,41 +273,15 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// x / (1 + 2^t) for two values, t clamped at 126 so that the denominator d
-// stays finite (the quotient is then below every 16-bit type's range).  The
-// reciprocal runs on the FMA pipe, two values an instruction: three Newton
-// steps r <- r + r (1 - d r) from a first guess read off the bits of d (the
-// integer 0x7EF311C3 - bits(d) is 1 / d within 11 %, and the error squares at
-// each step), which leaves one special-function operation a value: those
-// retire 16 a cycle and bounded the epilogue at two.
-__device__ __forceinline__ void quotient2(float& x0, float& x1, float t0,
-                                          float t1) {
-  asm("{\n\t"
-      ".reg .b64 X, ND, R, E, ONE;\n\t"
-      ".reg .b32 a0, a1, n0, n1, r0, r1;\n\t"
-      "mov.b64 ONE, {0x3F800000, 0x3F800000};\n\t"
-      "min.f32 a0, %2, 0f42FC0000;\n\t"  // 126
-      "min.f32 a1, %3, 0f42FC0000;\n\t"
-      "ex2.approx.ftz.f32 a0, a0;\n\t"
-      "ex2.approx.ftz.f32 a1, a1;\n\t"
-      "sub.rn.f32 n0, 0fBF800000, a0;\n\t"  // -d
-      "sub.rn.f32 n1, 0fBF800000, a1;\n\t"
-      "sub.u32 r0, 0xFEF311C3, n0;\n\t"
-      "sub.u32 r1, 0xFEF311C3, n1;\n\t"
-      "mov.b64 ND, {n0, n1};\n\t"
-      "mov.b64 R, {r0, r1};\n\t"
-      "mov.b64 X, {%0, %1};\n\t"
-      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
-      "fma.rn.f32x2 R, R, E, R;\n\t"
-      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
-      "fma.rn.f32x2 R, R, E, R;\n\t"
-      "fma.rn.f32x2 E, ND, R, ONE;\n\t"
-      "fma.rn.f32x2 R, R, E, R;\n\t"
-      "mul.rn.f32x2 X, X, R;\n\t"
-      "mov.b64 {%0, %1}, X;\n\t"
-      "}"
-      : "+f"(x0), "+f"(x1)
-      : "f"(t0), "f"(t1));
+// x / (1 + 2^t): two special-function operations, five instructions.  (The
+// reciprocal by Newton steps on the FMA pipe halves the former and doubles
+// the latter; the epilogue's few warps wait on instructions, not on that
+// pipe.)  For t > 127 the denominator is infinite and the quotient a zero.
+__device__ __forceinline__ float quotient(float x, float t) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return x * r;
 }
 
 // Not inlined: 32 copies of erfc would cost the epilogue its registers.
@@ -315,7 +289,7 @@ __device__ __noinline__ float gelu_erf(float x) {
   return 0.5f * x * erfcf(-0.7071067811865476f * x);
 }
 
-// act(v), NC values (an even number), in fp32.  silu(x) = x / (1 + e^-x);
+// act(v), NC values, in fp32.  silu(x) = x / (1 + e^-x);
 // 0.5 (1 + tanh u) = 1 / (1 + e^-2u), so the tanh form of gelu is
 // x / (1 + e^-2u) with u = sqrt(2/pi) (x + 0.044715 x^3); the erf form is
 // 0.5 x erfc(-x / sqrt 2), which keeps its digits for negative x.
@@ -328,15 +302,13 @@ __device__ __forceinline__ void activate(float (&v)[NC], int act) {
   } else if (act == NVFP4DG_ACT_SILU) {
     constexpr float k = -1.4426950408889634f;  // -log2(e)
 #pragma unroll
-    for (int i = 0; i < NC; i += 2)
-      quotient2(v[i], v[i + 1], k * v[i], k * v[i + 1]);
+    for (int i = 0; i < NC; ++i) v[i] = quotient(v[i], k * v[i]);
   } else if (act == NVFP4DG_ACT_GELU_TANH) {
     constexpr float k = -2.302208198201456f;  // -2 sqrt(2/pi) log2(e)
 #pragma unroll
-    for (int i = 0; i < NC; i += 2) {
-      const float x = v[i], y = v[i + 1];
-      quotient2(v[i], v[i + 1], k * x * fmaf(0.044715f, x * x, 1.f),
-                k * y * fmaf(0.044715f, y * y, 1.f));
+    for (int i = 0; i < NC; ++i) {
+      const float x = v[i];
+      v[i] = quotient(x, k * x * fmaf(0.044715f, x * x, 1.f));
     }
   } else {
 #pragma unroll
@@ -381,35 +353,53 @@ __device__ __forceinline__ float load_scale(const LinearParams& p, int x,
   return p.row_scale != nullptr && lane < nv ? p.row_scale[x + lane] : 0.f;
 }
 
-// Epilogue of NC rows (tokens) of one feature: the accumulators v to C.
-// `scale`: lane i holds the row scale of row i (NC <= 32).
-template <typename T, int NC>
-__device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
-                                       int nv, float bias, float scale,
-                                       const T (&r)[NC], float (&v)[NC]) {
+// NP of finish's rows, from its c-th.
+template <typename T, int NP, int NC>
+__device__ __forceinline__ void finish_part(const LinearParams& p, char* dst,
+                                            uint32_t off, uint32_t step,
+                                            int c, int nv, float bias,
+                                            float scale, const T (&r)[NC],
+                                            float (&v)[NC]) {
+  float(&w)[NP] = *reinterpret_cast<float(*)[NP]>(v + c);
 #pragma unroll
-  for (int i = 0; i < NC; ++i) v[i] = fmaf(p.alpha, v[i], bias);
-  activate<NC>(v, p.act);
+  for (int i = 0; i < NP; ++i) w[i] = fmaf(p.alpha, w[i], bias);
+  activate<NP>(w, p.act);
   if (p.row_scale != nullptr) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-      v[i] *= __shfl_sync(0xffffffffu, scale, i);
+    for (int i = 0; i < NP; ++i)
+      w[i] *= __shfl_sync(0xffffffffu, scale, c + i);
   }
   if (p.residual != nullptr) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) v[i] += to_f32<T>(r[i]);
+    for (int i = 0; i < NP; ++i) w[i] += to_f32<T>(r[c + i]);
   }
-  char* dst = static_cast<char*>(p.C) + (size_t)x * p.ldc * sizeof(T);
-  uint32_t off = n * sizeof(T);
-  const uint32_t step = p.ldc * sizeof(T);
-  if (nv >= NC) {
+  off += c * step;
 #pragma unroll
-    for (int i = 0; i < NC; ++i, off += step)
-      *reinterpret_cast<T*>(dst + off) = from_f32<T>(v[i]);
+  for (int i = 0; i < NP; ++i, off += step)
+    if (c + i < nv) *reinterpret_cast<T*>(dst + off) = from_f32<T>(w[i]);
+}
+
+// Epilogue of NC rows (tokens) of one feature: the accumulators v to C.  `cnt`
+// rows exist (the same for the whole warp), and `nv` of them are this
+// thread's: cnt, or none for a feature beyond N.  Lane i holds row i's scale.
+// All rows go at once (32 independent chains hide the latency of a warp that
+// has its scheduler almost to itself), or, where rows are missing, eight at a
+// time, so that a tile of few tokens does not pay for 32.
+template <typename T, int NC>
+__device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
+                                       int cnt, int nv, float bias,
+                                       float scale, const T (&r)[NC],
+                                       float (&v)[NC]) {
+  char* dst = static_cast<char*>(p.C) + (size_t)x * p.ldc * sizeof(T);
+  const uint32_t off = n * sizeof(T), step = p.ldc * sizeof(T);
+  if (NC <= 8 || cnt > NC - 8) {
+    finish_part<T, NC, NC>(p, dst, off, step, 0, nv, bias, scale, r, v);
   } else {
 #pragma unroll
-    for (int i = 0; i < NC; ++i, off += step)
-      if (i < nv) *reinterpret_cast<T*>(dst + off) = from_f32<T>(v[i]);
+    for (int c = 0; c < NC - 8; c += 8)
+      if (c < cnt)
+        finish_part<T, NC < 8 ? NC : 8, NC>(p, dst, off, step, c, nv, bias,
+                                            scale, r, v);
   }
 }
 
@@ -781,7 +771,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_ld_32cols(t_row + a * TN + 32 * c, v);
         tc_wait_ld();
         tie32(v);
-        finish<T, 32>(p, t.x0 + 32 * c, n, rows - 32 * c, bias, scale, r, v);
+        finish<T, 32>(p, t.x0 + 32 * c, n, cols - 32 * c, rows - 32 * c, bias,
+                      scale, r, v);
       }
       tc_fence_before();
       __syncwarp();
@@ -849,13 +840,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
         for (int o = group * kG; o < n_own; o += 2 * kG) {
           const int col = 4 * (g_own + o);
-          const int rows =
-              n < p.N ? min(nv - col, 4 * min(kG, n_own - o)) : 0;
+          const int cnt = min(nv - col, 4 * min(kG, n_own - o));
+          const int rows = n < p.N ? cnt : 0;
           T r[4 * kG];
           float v[4 * kG];
           load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
-          const float scale = load_scale(
-              p, t.x0 + col, min(nv - col, 4 * min(kG, n_own - o)), lane);
+          const float scale = load_scale(p, t.x0 + col, cnt, lane);
           __syncwarp();
           if constexpr (kG == 8) {
             tc_ld_32cols(t_row + col, v);
@@ -884,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          finish<T, 4 * kG>(p, t.x0 + col, n, rows, bias, scale, r, v);
+          finish<T, 4 * kG>(p, t.x0 + col, n, cnt, rows, bias, scale, r, v);
         }
       };
       if (n_own > 2)
