@@ -403,6 +403,95 @@ __device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
   }
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t u);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16),
+                     __uint_as_float(u & 0xFFFF0000u));
+}
+
+// The same epilogue where a thread is a token row: 32 columns of row x from
+// column n.
+template <typename T>
+__device__ __forceinline__ void load_residual_row(const LinearParams& p,
+                                                  int x, int n, bool live,
+                                                  uint4 (&r)[4]) {
+  if (p.residual == nullptr) return;
+  const T* src = static_cast<const T*>(p.residual) + (size_t)x * p.ldr + n;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    r[q] = make_uint4(0u, 0u, 0u, 0u);
+    if (live && n + 8 * q < p.N)
+      r[q] = *reinterpret_cast<const uint4*>(src + 8 * q);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void finish_row32(const LinearParams& p,
+                                             float scale, const float* bias,
+                                             const uint4 (&r)[4],
+                                             float (&v)[32], uint4 (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float4 b = reinterpret_cast<const float4*>(bias)[i];
+    v[4 * i + 0] = fmaf(p.alpha, v[4 * i + 0], b.x);
+    v[4 * i + 1] = fmaf(p.alpha, v[4 * i + 1], b.y);
+    v[4 * i + 2] = fmaf(p.alpha, v[4 * i + 2], b.z);
+    v[4 * i + 3] = fmaf(p.alpha, v[4 * i + 3], b.w);
+  }
+  activate<32>(v, p.act);
+  if (p.row_scale != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] *= scale;
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (p.residual != nullptr) {
+      const uint32_t w[4] = {r[q].x, r[q].y, r[q].z, r[q].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<T>(w[i]);
+        v[8 * q + 2 * i] += f.x;
+        v[8 * q + 2 * i + 1] += f.y;
+      }
+    }
+    o[q].x = pack2<T>(v[8 * q + 0], v[8 * q + 1]);
+    o[q].y = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
+    o[q].z = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
+    o[q].w = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
+  }
+}
+
+// Stores the first `cols` (a multiple of 8, 32 at most) of them.
+template <typename T>
+__device__ __forceinline__ void store_row32(const LinearParams& p, int x,
+                                            int n, bool live, int cols,
+                                            const uint4 (&o)[4]) {
+  T* dst = static_cast<T*>(p.C) + (size_t)x * p.ldc + n;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (live && n + 8 * q < p.N && 8 * q < cols)
+      *reinterpret_cast<uint4*>(dst + 8 * q) = o[q];
+  }
+}
+
 // A stage of linear_kernel's ring holds kSub blocks of 256 along K.  What a
 // stage costs beyond its bytes, a wait of ~300 cycles in each role and the MMA
 // thread's commit, made a 256-wide block take ~710 cycles; two of them at once
@@ -410,6 +499,10 @@ __device__ __forceinline__ void finish(const LinearParams& p, int x, int n,
 // as deep in bytes and one block wide.
 template <int TN>
 struct Cfg {
+  // 128 tokens: the tokens take the TMEM lanes and 128 features the columns,
+  // the other way round than with fewer.  A thread of the epilogue then holds
+  // a row's consecutive columns, which halves its instructions.
+  static constexpr bool kRows = TN == 128;
   static constexpr int kSub = TN <= 64 ? 2 : 1;
   static constexpr int kSteps = 4 * kSub;  // MMAs of 64 along K
   static constexpr int kWBox = kFeat * kRowBytes;
@@ -462,6 +555,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t recv_bar;
   __shared__ uint32_t tmem_base_sh;
   __shared__ GroupTable tab;
+  // kRows: the bias of a tile's features, for each epilogue group, by the
+  // accumulator's parity
+  __shared__ __align__(16) float
+      bias_sh[2][2][Cfg<TN>::kRows ? 128 + 32 : 4];
 
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
@@ -544,8 +641,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // block took ~1000 cycles whatever its size.
     {
       const bool w_side = warp == kProdWWarp;
-      const CUtensorMap* tm = w_side ? &tmW : &tmX;
-      const uint64_t pol = w_side ? kPolicyEvictNormal : kPolicyEvictLast;
+      // the 128 lanes' operand comes through the first producer
+      const bool weights = w_side != Cf::kRows;
+      const CUtensorMap* tm = weights ? &tmW : &tmX;
+      const uint64_t pol = weights ? kPolicyEvictNormal : kPolicyEvictLast;
       const uint32_t tile_off = w_side ? 0 : Cf::kWBytes;
       const uint32_t sf_off =
           Cf::kWBytes + Cf::kXBytes + (w_side ? 0 : Cf::kRun);
@@ -557,11 +656,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int tile = first; ok && tile < total; tile += step) {
         const Tile t = locate<TN>(p, tab, find, tile);  // the whole warp
         const uint8_t* sf =
-            w_side ? p.sfb + (size_t)t.g * p.sfb_group +
-                         (size_t)(t.n0 / 128) * kblk64 * kAtomBytes
-                   : p.sfa + (size_t)(t.x0 / 128) * kblk64 * kAtomBytes;
-        const int row = w_side ? t.n0 : t.x0;
-        const int layer = w_side ? t.g : 0;
+            weights ? p.sfb + (size_t)t.g * p.sfb_group +
+                          (size_t)(t.n0 / 128) * kblk64 * kAtomBytes
+                    : p.sfa + (size_t)(t.x0 / 128) * kblk64 * kAtomBytes;
+        const int row = weights ? t.n0 : t.x0;
+        const int layer = weights ? t.g : 0;
         for (int kb = kb0; lane == 0 && kb < kb1; ++kb) {
           if (issued >= S && !ready &&
               !mbar_wait(&empty_bar[stage], phase ^ 1u, p.err,
@@ -738,6 +837,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
     }
     __syncwarp();
+  } else if (Cf::kRows && p.split == 1) {
+    // ---------------------------------------------------------- epilogue
+    // A thread is a token row; the groups take chunks of 32 features in turn.
+    const int q = warp % 4, group = epi_group(warp);
+    const int row = 32 * q + lane;
+    const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16);
+    int it = 0;
+    griddep_wait();
+    for (int tile = first; tile < total; tile += step, ++it) {
+      const Tile t = locate<TN>(p, tab, find, tile);
+      const int a = it & 1;
+      const int x = t.x0 + row;
+      const bool live = row < t.rows;
+      const float scale =
+          p.row_scale != nullptr && live ? p.row_scale[x] : 0.f;
+      bias_sh[group][a][row] = load_bias<T>(p, t.g, t.n0 + row);
+      const bool got =
+          mbar_wait(&acc_full_bar[a], (it >> 1) & 1, p.err, kErrEpilogue);
+      if (!epi_all(group, got)) break;  // (and the bias is visible)
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = group; c < 4; c += 2) {
+        const int n = t.n0 + 32 * c;
+        if (n >= p.N) break;
+        float v[32];
+        uint4 r[4], o[4];
+        load_residual_row<T>(p, x, n, live, r);
+        __syncwarp();
+        tc_ld_32cols(t_row + a * TN + 32 * c, v);
+        tc_wait_ld();
+        tie32(v);
+        finish_row32<T>(p, scale, &bias_sh[group][a][32 * c], r, v, o);
+        store_row32<T>(p, x, n, live, 32, o);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty_bar[a]);
+    }
   } else if (p.split == 1) {
     // ---------------------------------------------------------- epilogue
     const int q = warp % 4, group = epi_group(warp);
@@ -787,9 +924,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const int row = 32 * q4 + lane;
     const Tile t = locate<TN>(p, tab, find, first);
-    const int nv = min(t.rows, TN);
+    // columns of the accumulator that are wanted: tokens, or features
+    const int nv = Cf::kRows ? min(p.N - t.n0, TN) : min(t.rows, TN);
     const int g4 = (nv + 3) / 4;
-    const int gpr = (g4 + p.split - 1) / p.split;
+    // (kRows: pieces in pairs, 16 bytes of a row)
+    const int gpr = Cf::kRows ? (g4 / 2 + p.split - 1) / p.split * 2
+                              : (g4 + p.split - 1) / p.split;
     const int g_own = rank * gpr;
     const int n_own = max(0, min(gpr, g4 - g_own));
     const uint32_t recv = smem_u32(smem + S * Cf::kStageBytes);
@@ -798,6 +938,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_wait();
     const int n = t.n0 + row;
     const float bias = load_bias<T>(p, t.g, n);
+    if (Cf::kRows) {
+      // (32 more: a chunk of 32 columns may reach past the rank's share)
+      bias_sh[group][0][row] = bias;
+      if (row < 32) bias_sh[group][0][128 + row] = 0.f;
+      epi_bar(group);
+    }
     const bool got = mbar_wait(&acc_full_bar[0], 0, p.err, kErrEpilogue);
     if (__all_sync(0xffffffffu, got)) {
       tc_fence_after();
@@ -841,11 +987,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int o = group * kG; o < n_own; o += 2 * kG) {
           const int col = 4 * (g_own + o);
           const int cnt = min(nv - col, 4 * min(kG, n_own - o));
-          const int rows = n < p.N ? cnt : 0;
-          T r[4 * kG];
-          float v[4 * kG];
-          load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
-          const float scale = load_scale(p, t.x0 + col, cnt, lane);
+          [[maybe_unused]] const int rows = n < p.N ? cnt : 0;
+          [[maybe_unused]] const int x = t.x0 + row;  // (kRows)
+          [[maybe_unused]] const bool live = row < t.rows;
+          [[maybe_unused]] T r[Cf::kRows ? 1 : 4 * kG];
+          [[maybe_unused]] uint4 rr[4];
+          float v[4 * kG], scale;
+          if constexpr (Cf::kRows) {
+            load_residual_row<T>(p, x, t.n0 + col, live, rr);
+            scale = p.row_scale != nullptr && live ? p.row_scale[x] : 0.f;
+          } else {
+            load_residual<T, 4 * kG>(p, t.x0 + col, n, rows, r);
+            scale = load_scale(p, t.x0 + col, cnt, lane);
+          }
           __syncwarp();
           if constexpr (kG == 8) {
             tc_ld_32cols(t_row + col, v);
@@ -874,13 +1028,24 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          finish<T, 4 * kG>(p, t.x0 + col, n, cnt, rows, bias, scale, r, v);
+          if constexpr (Cf::kRows) {
+            uint4 out[4];
+            finish_row32<T>(p, scale, &bias_sh[group][0][col], rr, v, out);
+            store_row32<T>(p, x, t.n0 + col, live, cnt, out);
+          } else {
+            finish<T, 4 * kG>(p, t.x0 + col, n, cnt, rows, bias, scale, r,
+                              v);
+          }
         }
       };
-      if (n_own > 2)
+      if constexpr (Cf::kRows) {
         share(std::integral_constant<int, 8>());
-      else
-        share(std::integral_constant<int, 1>());
+      } else {
+        if (n_own > 2)
+          share(std::integral_constant<int, 8>());
+        else
+          share(std::integral_constant<int, 1>());
+      }
     }
   }
 
@@ -955,72 +1120,6 @@ __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
   t.rows = rows - m0;
   t.sfa_last = (row0 + rows - 1) / 128;
   return t;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t u);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&u));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
-  return make_float2(__uint_as_float(u << 16),
-                     __uint_as_float(u & 0xFFFF0000u));
-}
-
-// Epilogue of 32 columns of one row from column n: accumulators v to packed
-// outputs o.
-template <typename T>
-__device__ __forceinline__ void finish_row32(const LinearParams& p, int x,
-                                             int n, bool live, float scale,
-                                             const float* bias, float (&v)[32],
-                                             uint4 (&o)[4]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float4 b = reinterpret_cast<const float4*>(bias)[i];
-    v[4 * i + 0] = fmaf(p.alpha, v[4 * i + 0], b.x);
-    v[4 * i + 1] = fmaf(p.alpha, v[4 * i + 1], b.y);
-    v[4 * i + 2] = fmaf(p.alpha, v[4 * i + 2], b.z);
-    v[4 * i + 3] = fmaf(p.alpha, v[4 * i + 3], b.w);
-  }
-  activate<32>(v, p.act);
-  if (p.row_scale != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= scale;
-  }
-  const T* res = p.residual == nullptr
-                     ? nullptr
-                     : static_cast<const T*>(p.residual) + (size_t)x * p.ldr;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (res != nullptr && live && n + 8 * q < p.N) {
-      const uint4 r = *reinterpret_cast<const uint4*>(res + n + 8 * q);
-      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(w[i]);
-        v[8 * q + 2 * i] += f.x;
-        v[8 * q + 2 * i + 1] += f.y;
-      }
-    }
-    o[q].x = pack2<T>(v[8 * q + 0], v[8 * q + 1]);
-    o[q].y = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
-    o[q].z = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
-    o[q].w = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
-  }
 }
 
 template <typename T>
@@ -1350,6 +1449,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int ph = 0; ph < 2; ++ph) {
         const int n = n0 + 64 * ph;
         float v[2][32];
+        uint4 res[2][4];
+        load_residual_row<T>(p, x, n, live, res[0]);
+        load_residual_row<T>(p, x, n + 32, live, res[1]);
         __syncwarp();
         tc_ld_32cols(t_row + 128 * group + 64 * ph, v[0]);
         tc_ld_32cols(t_row + 128 * group + 64 * ph + 32, v[1]);
@@ -1370,18 +1472,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint4 o[4];
-          finish_row32<T>(p, x, n + 32 * h, live, scale,
-                          bias + 64 * ph + 32 * h, v[h], o);
+          finish_row32<T>(p, scale, bias + 64 * ph + 32 * h, res[h], v[h], o);
+          if (boxed) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (boxed)
+            for (int q = 0; q < 4; ++q)
               sts128(smem_u32(box + row * 128 +
                               (((4 * h + q) ^ (row & 7)) << 4)),
                      o[q]);
-            else if (live && n + 32 * h + 8 * q < p.N)
-              *reinterpret_cast<uint4*>(static_cast<T*>(p.C) +
-                                        (size_t)x * p.ldc + n + 32 * h +
-                                        8 * q) = o[q];
+          } else {
+            store_row32<T>(p, x, n + 32 * h, live, 32, o);
           }
         }
         if (boxed) {

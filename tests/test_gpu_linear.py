@@ -57,7 +57,8 @@ class Problem:
 @pytest.mark.parametrize("m,n,k", [(1, 8, 64), (33, 136, 2368),
                                    (130, 264, 2048)])
 def test_every_schedule(m, n, k, tile, split):
-    p = Problem(m, n, k, seed=m + n + k, residual=True, bias=torch.float32)
+    p = Problem(m, n, k, seed=m + n + k, residual=True, bias=torch.float32,
+                row_scale=True)
     flags = TILES[tile] | (_lib.linear_split(split) if split else 0)
     p.check(p.run(flags=flags), f"{tile} split {split}")
 
@@ -76,6 +77,9 @@ def test_columns(m, n):
     p = Problem(m, n, 320, seed=n, residual=True)
     p.check(p.run(), f"n {n}")
     p.check(p.run(flags=_lib.LINEAR_PAIR), f"pair, n {n}")
+    for split in (1, 2):
+        p.check(p.run(flags=_lib.LINEAR_TOKENS128 | _lib.linear_split(split)),
+                f"t128 split {split}, n {n}")
 
 
 @pytest.mark.parametrize("k", [64, 128, 192, 256, 320, 448, 512, 1088, 4096])
