@@ -94,30 +94,20 @@ __device__ __forceinline__ int group_rows(const LinearParams& p, int g,
   return min(max(n, 0), p.M - row0);
 }
 
-// A tile's place among the groups, found by a whole warp: each lane holds the
-// first tiles of groups lane, lane + 32, ... in registers, and the groups that
-// start at or below the tile are counted by votes.  (A search of the table in
-// shared memory by the one thread that needs it took ~1500 cycles a tile, as
-// long as a tile of short K.)
-struct GroupFinder {
-  int tile0[kMaxGroups / 32];
-  __device__ __forceinline__ void set(const LinearParams& p,
-                                      const GroupTable& tab, int lane) {
-#pragma unroll
-    for (int k = 0; k < kMaxGroups / 32; ++k)
-      tile0[k] = 32 * k + lane < p.groups ? tab.tile0[32 * k + lane]
-                                          : 0x7fffffff;
-  }
-  // the last group whose first tile is <= tile (empty groups have none)
-  __device__ __forceinline__ int find(const LinearParams& p, int tile) const {
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < kMaxGroups / 32; ++k)
-      if (32 * k < p.groups)
-        n += __popc(__ballot_sync(0xffffffffu, tile0[k] <= tile));
-    return n - 1;
-  }
-};
+// The last group whose first tile is <= tile (empty groups have none), found
+// by a whole warp: each lane looks at groups lane, lane + 32, ..., and the
+// groups that start at or below the tile are counted by votes.  (A search by
+// the one thread that needs it took ~1500 cycles a tile, as long as a tile of
+// short K.)
+__device__ __forceinline__ int find_group(const LinearParams& p,
+                                          const GroupTable& tab, int tile) {
+  const int lane = threadIdx.x % 32;
+  int n = 0;
+  for (int g = lane; g - lane < p.groups; g += 32)
+    n += __popc(__ballot_sync(0xffffffffu,
+                              g < p.groups && tab.tile0[g] <= tile));
+  return n - 1;
+}
 
 struct Tile {
   int g;       // group (batch of B)
@@ -178,8 +168,7 @@ __device__ __forceinline__ void build_groups(const LinearParams& p, int tn,
 // weights at the same time.  Called by whole warps.
 template <int TN>
 __device__ __forceinline__ Tile locate(const LinearParams& p,
-                                       const GroupTable& tab,
-                                       const GroupFinder& find, int tile) {
+                                       const GroupTable& tab, int tile) {
   Tile t;
   if (p.groups == 0) {
     const int nt = p.m_tiles == 1 ? tile : tile / p.m_tiles;
@@ -189,7 +178,7 @@ __device__ __forceinline__ Tile locate(const LinearParams& p,
     t.rows = p.M - t.x0;
     return t;
   }
-  const int g = find.find(p, tile);
+  const int g = find_group(p, tab, tile);
   const int local = tile - tab.tile0[g];
   const int row0 = tab.row0[g];
   const int rows = group_rows(p, g, row0);
@@ -217,6 +206,52 @@ __device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+// A counter in shared memory that one thread of the CTA raises and another
+// waits for (release and acquire, so what the first saw the second sees);
+// bounded as mbar_wait is.
+__device__ __forceinline__ void flag_set(uint32_t* flag, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(
+                   smem_u32(flag)),
+               "r"(v)
+               : "memory");
+}
+__device__ __forceinline__ bool flag_wait(uint32_t* flag, uint32_t target,
+                                          unsigned* err, unsigned code) {
+  long long t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t v;
+    asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];"
+                 : "=r"(v)
+                 : "r"(smem_u32(flag))
+                 : "memory");
+    if (static_cast<int32_t>(v - target) >= 0) return true;
+    if ((i & 4095u) == 0u) {
+      const long long now = clock_cycles();
+      if (t0 == 0) t0 = now;
+      const bool gone = *reinterpret_cast<volatile unsigned*>(err) != 0u;
+      if (gone || now - t0 > kWaitLimitCycles) {
+        if (!gone) atomicOr(err, code);
+        note_wait_failed();
+        return false;
+      }
+    }
+  }
+}
+
+// Arrives on `bar` of both CTAs of the pair when this thread's 2-SM MMAs are
+// done.
+__device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster."
+      "multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 
 // 4 consecutive 32-bit TMEM columns of this warp's 32 lanes.
@@ -443,11 +478,13 @@ __device__ __forceinline__ void load_residual_row(const LinearParams& p,
   }
 }
 
-template <typename T>
+// `residual(q)` gives its eight elements from column 8 q, `emit(q, o)` takes
+// the outputs there.
+template <typename T, typename R, typename E>
 __device__ __forceinline__ void finish_row32(const LinearParams& p,
                                              float scale, const float* bias,
-                                             const uint4 (&r)[4],
-                                             float (&v)[32], uint4 (&o)[4]) {
+                                             float (&v)[32], R residual,
+                                             E emit) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float4 b = reinterpret_cast<const float4*>(bias)[i];
@@ -464,7 +501,8 @@ __device__ __forceinline__ void finish_row32(const LinearParams& p,
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     if (p.residual != nullptr) {
-      const uint32_t w[4] = {r[q].x, r[q].y, r[q].z, r[q].w};
+      const uint4 r = residual(q);
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = unpack2<T>(w[i]);
@@ -472,24 +510,18 @@ __device__ __forceinline__ void finish_row32(const LinearParams& p,
         v[8 * q + 2 * i + 1] += f.y;
       }
     }
-    o[q].x = pack2<T>(v[8 * q + 0], v[8 * q + 1]);
-    o[q].y = pack2<T>(v[8 * q + 2], v[8 * q + 3]);
-    o[q].z = pack2<T>(v[8 * q + 4], v[8 * q + 5]);
-    o[q].w = pack2<T>(v[8 * q + 6], v[8 * q + 7]);
+    emit(q, make_uint4(pack2<T>(v[8 * q + 0], v[8 * q + 1]),
+                       pack2<T>(v[8 * q + 2], v[8 * q + 3]),
+                       pack2<T>(v[8 * q + 4], v[8 * q + 5]),
+                       pack2<T>(v[8 * q + 6], v[8 * q + 7])));
   }
 }
 
-// Stores the first `cols` (a multiple of 8, 32 at most) of them.
+// Eight outputs of row x from column n.
 template <typename T>
-__device__ __forceinline__ void store_row32(const LinearParams& p, int x,
-                                            int n, bool live, int cols,
-                                            const uint4 (&o)[4]) {
-  T* dst = static_cast<T*>(p.C) + (size_t)x * p.ldc + n;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (live && n + 8 * q < p.N && 8 * q < cols)
-      *reinterpret_cast<uint4*>(dst + 8 * q) = o[q];
-  }
+__device__ __forceinline__ void store_row8(const LinearParams& p, int x, int n,
+                                           const uint4& o) {
+  *reinterpret_cast<uint4*>(static_cast<T*>(p.C) + (size_t)x * p.ldc + n) = o;
 }
 
 // A stage of linear_kernel's ring holds kSub blocks of 256 along K.  What a
@@ -626,8 +658,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int total =
       p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
-  GroupFinder find;
-  if (p.groups > 0) find.set(p, tab, lane);
   const int first = static_cast<int>(blockIdx.x) / p.split;
   const int step = static_cast<int>(gridDim.x) / p.split;
   const int kb0 = static_cast<int>((long long)p.kblocks * rank / p.split);
@@ -654,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true, ready = false;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
-        const Tile t = locate<TN>(p, tab, find, tile);  // the whole warp
+        const Tile t = locate<TN>(p, tab, tile);  // the whole warp
         const uint8_t* sf =
             weights ? p.sfb + (size_t)t.g * p.sfb_group +
                           (size_t)(t.n0 / 128) * kblk64 * kAtomBytes
@@ -712,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_wait();
     for (int tile = first; ok && tile < total; tile += step) {
       const int part =
-          TN == 128 ? 0 : (locate<TN>(p, tab, find, tile).x0 % 128) / 32;
+          TN == 128 ? 0 : (locate<TN>(p, tab, tile).x0 % 128) / 32;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!__all_sync(0xffffffffu, ready)) {
           const bool got =
@@ -846,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, ++it) {
-      const Tile t = locate<TN>(p, tab, find, tile);
+      const Tile t = locate<TN>(p, tab, tile);
       const int a = it & 1;
       const int x = t.x0 + row;
       const bool live = row < t.rows;
@@ -862,14 +892,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = t.n0 + 32 * c;
         if (n >= p.N) break;
         float v[32];
-        uint4 r[4], o[4];
+        uint4 r[4];
         load_residual_row<T>(p, x, n, live, r);
         __syncwarp();
         tc_ld_32cols(t_row + a * TN + 32 * c, v);
         tc_wait_ld();
         tie32(v);
-        finish_row32<T>(p, scale, &bias_sh[group][a][32 * c], r, v, o);
-        store_row32<T>(p, x, n, live, 32, o);
+        finish_row32<T>(
+            p, scale, &bias_sh[group][a][32 * c], v,
+            [&](int i) { return r[i]; },
+            [&](int i, const uint4& o) {
+              if (live && n + 8 * i < p.N) store_row8<T>(p, x, n + 8 * i, o);
+            });
       }
       tc_fence_before();
       __syncwarp();
@@ -882,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int it = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, ++it) {
-      const Tile t = locate<TN>(p, tab, find, tile);
+      const Tile t = locate<TN>(p, tab, tile);
       const int a = it & 1;
       const int n = t.n0 + 32 * q + lane;
       const float bias = load_bias<T>(p, t.g, n);
@@ -923,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q4 = warp % 4, group = epi_group(warp);
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
     const int row = 32 * q4 + lane;
-    const Tile t = locate<TN>(p, tab, find, first);
+    const Tile t = locate<TN>(p, tab, first);
     // columns of the accumulator that are wanted: tokens, or features
     const int nv = Cf::kRows ? min(p.N - t.n0, TN) : min(t.rows, TN);
     const int g4 = (nv + 3) / 4;
@@ -1029,9 +1063,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           if constexpr (Cf::kRows) {
-            uint4 out[4];
-            finish_row32<T>(p, scale, &bias_sh[group][0][col], rr, v, out);
-            store_row32<T>(p, x, t.n0 + col, live, cnt, out);
+            finish_row32<T>(
+                p, scale, &bias_sh[group][0][col], v,
+                [&](int i) { return rr[i]; },
+                [&](int i, const uint4& out) {
+                  if (live && 8 * i < cnt)
+                    store_row8<T>(p, x, t.n0 + col + 8 * i, out);
+                });
           } else {
             finish<T, 4 * kG>(p, t.x0 + col, n, cnt, rows, bias, scale, r,
                               v);
@@ -1070,6 +1108,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // token row; outputs leave through shared memory and TMA stores, 64 columns
 // at a time.
 // ---------------------------------------------------------------------------
+constexpr int kPairThreads = 512;
+constexpr int kPairWaiter = 15;   // see below
 constexpr int kPairStages = 5;
 constexpr int kPairTile = 128 * kRowBytes;  // one CTA's token or weight rows
 constexpr int kPairStageBytes = 2 * kPairTile + 3 * kRunBytes;
@@ -1091,7 +1131,6 @@ struct PairTile {
 // operand rows than whole columns of m tiles do.
 __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
                                                 const GroupTable& tab,
-                                                const GroupFinder& find,
                                                 int tile) {
   PairTile t;
   if (p.groups == 0) {
@@ -1107,7 +1146,7 @@ __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
     t.sfa_last = (p.M - 1) / 128;
     return t;
   }
-  const int g = find.find(p, tile);
+  const int g = find_group(p, tab, tile);
   const int local = tile - tab.tile0[g];
   const int row0 = tab.row0[g];
   const int rows = group_rows(p, g, row0);
@@ -1123,7 +1162,7 @@ __device__ __forceinline__ PairTile locate_pair(const LinearParams& p,
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmW,
                        const __grid_constant__ CUtensorMap tmX,
                        const __grid_constant__ CUtensorMap tmC,
@@ -1137,6 +1176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t acc_empty_bar;
   __shared__ __align__(8) uint64_t drain_bar;
   __shared__ uint32_t tmem_base_sh;
+  __shared__ uint32_t landed_sh;  // K blocks ready for the MMA thread
   __shared__ __align__(16) float bias_sh[256];
   __shared__ GroupTable tab;
 
@@ -1175,7 +1215,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar, count);
       fence_mbar_init();
     }
-    if (lane == 0) s_wait_failed = 0u;
+    if (lane == 0) {
+      s_wait_failed = 0u;
+      landed_sh = 0u;
+    }
     if (lane == 29) prefetch_tmap(&tmW);
     if (lane == 30) prefetch_tmap(&tmX);
     if (lane == 31) prefetch_tmap(&tmC);
@@ -1201,8 +1244,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_base_sh;
   const int total =
       p.groups > 0 ? tab.tile0[p.groups] : p.n_tiles * p.m_tiles;
-  GroupFinder find;
-  if (p.groups > 0) find.set(p, tab, lane);
   const int first = static_cast<int>(blockIdx.x) / 2;
   const int step = static_cast<int>(gridDim.x) / 2;
 
@@ -1218,10 +1259,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0;
       uint32_t phase = 0;
       long long issued = 0;
-      bool ok = true, ready = false;
+      bool ok = true;
       griddep_wait();  // global memory only after the previous grid
       for (int tile = first; ok && tile < total; tile += step) {
-        const PairTile t = locate_pair(p, tab, find, tile);
+        const PairTile t = locate_pair(p, tab, tile);
         const int row = (x_side ? t.x0 : t.n0) + 128 * static_cast<int>(rank);
         // the odd CTA's rows may lie past the problem's last row block, and
         // the second weight run past the last one: they copy the last, whose
@@ -1235,7 +1276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                              (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
                                  kAtomBytes;
         for (int kb = 0; lane == 0 && kb < p.kblocks; ++kb) {
-          if (issued >= S && !ready &&
+          if (issued >= S &&
               !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
                                  kErrProducer)) {
             ok = false;
@@ -1243,17 +1284,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const int next = stage + 1 == S ? 0 : stage + 1;
           const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
-          ready = mbar_peek(&empty_bar[next], next_phase ^ 1u);
           uint8_t* st = smem + stage * kPairStageBytes;
           uint8_t* sf = st + 2 * kPairTile;
           const size_t run =
               (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes;
           const uint32_t full_s = full_c + 8u * static_cast<uint32_t>(stage);
           if (x_side) {
-            // the MMAs that read this stage in both CTAs are done: pass that
-            // on to the odd CTA
-            if (leader && issued >= S)
-              mbar_arrive_cluster(mapa_shared(smem_u32(&empty_bar[stage]), 1));
             bulk_load(sf, sfa + run, run_bytes, &sfdata_bar[stage], pol);
             bulk_load(sf + kRunBytes, sfb + run, run_bytes,
                       &sfdata_bar[stage], pol);
@@ -1270,6 +1306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
+      const bool ok_all = ok;
       // never leave with copies in flight: scale runs land on this CTA's
       // barriers, both CTAs' tiles on the even one's
       for (int s = 0; s < S; ++s) {
@@ -1279,6 +1316,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_wait(&sfdata_bar[s], par, p.err, kErrDrain, false);
           if (x_side && leader)
             mbar_wait_cluster(&full_bar[s], par, p.err, kErrDrain, false);
+          // the stage's last commit, which the even CTA sends to both: none
+          // may be on its way when a CTA leaves
+          if (ok_all)
+            mbar_wait_cluster(&empty_bar[s], par, p.err, kErrDrain, false);
         }
       }
     }
@@ -1289,21 +1330,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t t_lane = tmem + ((32u * q) << 16);
     int stage = 0;
     uint32_t phase = 0;
-    bool ok = true, ready = false;
+    bool ok = true;
     griddep_wait();
     for (int tile = first; ok && tile < total; tile += step) {
       for (int kb = 0; kb < p.kblocks; ++kb) {
-        if (!__all_sync(0xffffffffu, ready)) {
-          const bool got =
-              mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
-          if (!__all_sync(0xffffffffu, got)) {
-            ok = false;
-            break;
-          }
+        const bool got = mbar_wait(&sfdata_bar[stage], phase, p.err, kErrMma);
+        if (!__all_sync(0xffffffffu, got)) {
+          ok = false;
+          break;
         }
         const int next = stage + 1 == S ? 0 : stage + 1;
         const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
-        ready = mbar_peek(&sfdata_bar[next], next_phase);
         // arm the stage's next fill: it cannot complete before all four
         // scale warps have passed this one
         if (warp == kSfWarp0 && lane == 0)
@@ -1360,8 +1397,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t w_desc0 = smem_desc(smem_u32(smem) + kPairTile, 16, 1024,
                                          SmemLayout::kSwizzle128B);
       int stage = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true, any = false, ready = false;
+      uint32_t acc_phase = 0, block = 0;
+      bool ok = true, any = false;
       for (int tile = first; ok && tile < total; tile += step) {
         if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
                                kErrMma)) {
@@ -1370,14 +1407,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!ready &&
-              !mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
+          if (!flag_wait(&landed_sh, ++block, p.err, kErrMma)) {
             ok = false;
             break;
           }
           const int next = stage + 1 == S ? 0 : stage + 1;
-          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
-          ready = mbar_peek(&full_bar[next], next_phase);
           tc_fence_after();
           const uint32_t soff =
               static_cast<uint32_t>(stage) * (kPairStageBytes >> 4);
@@ -1395,14 +1429,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                                w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
                                sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
           }
-          tc_commit_pair(mapa_shared(smem_u32(&empty_bar[stage]), 0));
+          tc_commit_both(&empty_bar[stage]);
           any = true;
           stage = next;
-          phase = next_phase;
         }
         if (!ok) break;
-        tc_commit_pair(mapa_shared(smem_u32(&acc_full_bar), 0));
-        tc_commit_pair(mapa_shared(smem_u32(&acc_full_bar), 1));
+        tc_commit_both(&acc_full_bar);
         acc_phase ^= 1u;
       }
       // the last release of the accumulator (the odd CTA's warps arrive here
@@ -1412,6 +1444,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err, kErrMma);
       tc_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
       mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
+    }
+    __syncwarp();
+  } else if (warp == kPairWaiter) {
+    // ---------------------------------------------------------- waiter
+    // Waits for each K block's barrier in the MMA thread's stead and counts
+    // the blocks in shared memory, where that thread reads the count in a few
+    // cycles: its own wait would keep the tensor cores idle for ~300 cycles a
+    // block of 512.
+    if (lane == 0 && leader) {
+      int stage = 0;
+      uint32_t phase = 0, block = 0;
+      bool ok = true;
+      for (int tile = first; ok && tile < total; tile += step) {
+        for (int kb = 0; kb < p.kblocks; ++kb) {
+          if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
+            ok = false;
+            break;
+          }
+          flag_set(&landed_sh, ++block);
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
     }
     __syncwarp();
   } else {
@@ -1428,7 +1485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t acc_phase = 0;
     griddep_wait();
     for (int tile = first; tile < total; tile += step, acc_phase ^= 1u) {
-      const PairTile t = locate_pair(p, tab, find, tile);
+      const PairTile t = locate_pair(p, tab, tile);
       const int rows = t.rows - 128 * static_cast<int>(rank);  // of this CTA
       const int x = t.x0 + 128 * static_cast<int>(rank) + row;
       const bool live = row < rows;
@@ -1437,6 +1494,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n0 = t.n0 + 128 * group;
       epi_bar(group);  // the previous tile's bias has been read
       bias[row] = load_bias<T>(p, t.g, n0 + row);
+      if (p.residual != nullptr && live) {
+        // the row's 256 bytes, to L2 while the products run
+        const T* r =
+            static_cast<const T*>(p.residual) + (size_t)x * p.ldr + n0;
+        for (int i = 0; i < 128 && n0 + i < p.N; i += 64) prefetch_l2(r + i);
+      }
       const bool got =
           mbar_wait_cluster(&acc_full_bar, acc_phase, p.err, kErrEpilogue);
       // the four warps leave together: they meet at the barriers below
@@ -1471,17 +1534,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint4 o[4];
-          finish_row32<T>(p, scale, bias + 64 * ph + 32 * h, res[h], v[h], o);
-          if (boxed) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              sts128(smem_u32(box + row * 128 +
-                              (((4 * h + q) ^ (row & 7)) << 4)),
-                     o[q]);
-          } else {
-            store_row32<T>(p, x, n + 32 * h, live, 32, o);
-          }
+          finish_row32<T>(
+              p, scale, bias + 64 * ph + 32 * h, v[h],
+              [&](int i) { return res[h][i]; },
+              [&](int i, const uint4& o) {
+                if (boxed)
+                  sts128(smem_u32(box + row * 128 +
+                                  (((4 * h + i) ^ (row & 7)) << 4)),
+                         o);
+                else if (live && n + 32 * h + 8 * i < p.N)
+                  store_row8<T>(p, x, n + 32 * h + 8 * i, o);
+              });
         }
         if (boxed) {
           fence_proxy_async_smem();
@@ -1639,7 +1702,7 @@ int launch_pair(const LinearParams& kp, const LinearPlan& pl,
   p.n_tiles = (p.N + 255) / 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.grid, 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
