@@ -294,7 +294,8 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
 /* flags of nvfp4_linear_args (0 = automatic), beside
  * NVFP4DG_FLAG_SYNC_CHECK and NVFP4DG_FLAG_NO_PDL: the tokens a tile holds
  * and how many CTAs share a tile's K range (bits 8-10: 1 + log2, 0 =
- * automatic; not for grouped products). */
+ * automatic; at most one for each K block of 256 or, up to 64 tokens, 512;
+ * not for grouped products or pairs, which ignore it). */
 #define NVFP4DG_LINEAR_TOKENS32 (1u << 0)
 #define NVFP4DG_LINEAR_TOKENS64 (1u << 1)
 #define NVFP4DG_LINEAR_TOKENS128 (1u << 2)
@@ -343,11 +344,13 @@ NVFP4DG_API int nvfp4_linear_run_grouped(const nvfp4_linear_args* args,
                                          const int* group_row0, int groups,
                                          int on_device, void* stream);
 
-/* The schedule nvfp4_linear_run would use: tokens per tile, CTAs per tile
- * and CTAs in all.  Any out pointer may be NULL.  Host-only. */
-NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, unsigned flags,
-                                  int num_sms, int* tokens_out,
-                                  int* split_out, int* grid_out);
+/* The schedule nvfp4_linear_run would use, with a residual (`residual` != 0)
+ * or without: tokens per tile (256: 2-SM pairs), CTAs that share a tile's K
+ * range, and CTAs in all.  Any out pointer may be NULL.  Host-only. */
+NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, int residual,
+                                  unsigned flags, int num_sms,
+                                  int* tokens_out, int* split_out,
+                                  int* grid_out);
 
 /*
  * Norms between two blocks of a transformer, fused with the gate and scale

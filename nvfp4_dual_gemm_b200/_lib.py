@@ -114,7 +114,7 @@ SIGNATURES = {
     "nvfp4_linear_run": (_i, [ctypes.POINTER(LinearArgs), _vp]),
     "nvfp4_linear_run_grouped": (_i, [ctypes.POINTER(LinearArgs), _vp, _vp,
                                       _i, _i, _vp]),
-    "nvfp4_linear_plan": (_i, [_i, _i, _i, _u, _i, _ip, _ip, _ip]),
+    "nvfp4_linear_plan": (_i, [_i, _i, _i, _i, _u, _i, _ip, _ip, _ip]),
     "nvfp4_block_norm_run": (_i, [ctypes.POINTER(BlockNormArgs), _vp]),
     "nvfp4_quantize": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp]),
     "nvfp4_quantize_rows": (_i, [_vp, _i, _i, _i, ctypes.c_longlong, _vp, _vp,

@@ -303,10 +303,8 @@ def linear(A, B, SFA, SFB, C=None, *, bias=None, activation=None,
     workspace and can be captured into a CUDA graph; inference only
     (``nvfp4_linear_run``).  For one token up to a few the CTAs of a cluster
     share each tile's K range; the result does not depend on timing."""
-    return _lib.ext().linear(A, B, SFA, SFB, C, bias=bias,
-                             activation=activation, residual=residual,
-                             row_scale=row_scale, alpha=alpha, dtype=dtype,
-                             flags=flags)
+    return _lib.ext().linear(A, B, SFA, SFB, C, bias, activation, residual,
+                             row_scale, alpha, dtype, flags)
 
 
 def linear_grouped(A, B, SFA, SFB, C, group_rows, group_row0=None, *,
@@ -327,19 +325,20 @@ def linear_grouped(A, B, SFA, SFB, C, group_rows, group_row0=None, *,
     group that is out of place is empty and one that reaches past the rows of
     A or C is cut there (``nvfp4_linear_run_grouped``)."""
     return _lib.ext().linear_grouped(A, B, SFA, SFB, C, group_rows,
-                                     group_row0, bias=bias,
-                                     activation=activation,
-                                     row_scale=row_scale, alpha=alpha,
-                                     flags=flags)
+                                     group_row0, bias, activation, row_scale,
+                                     alpha, flags)
 
 
-def linear_plan(M: int, N: int, K: int, flags: int = 0,
-                num_sms: int = 148) -> dict:
-    """The schedule :func:`linear` would use (host-only; needs no GPU)."""
+def linear_plan(M: int, N: int, K: int, residual: bool = False,
+                flags: int = 0, num_sms: int = 148) -> dict:
+    """The schedule :func:`linear` would use, with a residual or without:
+    tokens per tile (256: 2-SM pairs), CTAs that share a tile's K range
+    (``split``) and CTAs in all (host-only; needs no GPU)."""
     lib = _lib.load()
     tokens, split, grid = (ctypes.c_int() for _ in range(3))
-    rc = lib.nvfp4_linear_plan(M, N, K, flags, num_sms, ctypes.byref(tokens),
-                               ctypes.byref(split), ctypes.byref(grid))
+    rc = lib.nvfp4_linear_plan(M, N, K, int(residual), flags, num_sms,
+                               ctypes.byref(tokens), ctypes.byref(split),
+                               ctypes.byref(grid))
     _lib.check(rc, "nvfp4_linear_plan")
     return {"tokens": tokens.value, "split": split.value, "grid": grid.value}
 
@@ -364,11 +363,9 @@ def block_norm(x, y=None, *, weight=None, bias=None, post_weight=None,
     rows for one a row.  ``R`` and ``Z`` are allocated when not given; R may
     be x or y.  [rows, D] tensors may have strided rows (16-byte pitches).
     D % 8 == 0 up to 32768.  Inference only (``nvfp4_block_norm_run``)."""
-    return _lib.ext().block_norm(x, y, weight=weight, bias=bias,
-                                 post_weight=post_weight,
-                                 post_bias=post_bias, gate=gate, scale=scale,
-                                 kind=kind, eps=eps, post=post, pre=pre, R=R,
-                                 Z=Z, flags=flags)
+    return _lib.ext().block_norm(x, y, weight, bias, post_weight, post_bias,
+                                 gate, scale, kind, eps, post, pre, R, Z,
+                                 flags)
 
 
 def block_norm_nvfp4(x, y=None, *, weight=None, bias=None, post_weight=None,
@@ -379,11 +376,9 @@ def block_norm_nvfp4(x, y=None, *, weight=None, bias=None, post_weight=None,
     (:func:`dual_gemm`, :func:`linear`): returns (R, codes [rows, D/2],
     blocked scales), equal bit for bit to :func:`quantize_nvfp4` of
     :func:`block_norm`'s Z, which is never written.  D % 64 == 0."""
-    return _lib.ext().block_norm_nvfp4(x, y, weight=weight, bias=bias,
-                                       post_weight=post_weight,
-                                       post_bias=post_bias, gate=gate,
-                                       scale=scale, kind=kind, eps=eps,
-                                       post=post, R=R, flags=flags)
+    return _lib.ext().block_norm_nvfp4(x, y, weight, bias, post_weight,
+                                       post_bias, gate, scale, kind, eps,
+                                       post, R, flags)
 
 
 def host_staging_size(M: int, N: int, K: int) -> int:

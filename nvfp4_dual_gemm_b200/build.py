@@ -127,7 +127,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
            *[f"-I{d}" for d in incs], EXT_SOURCE, "-o", tmp,
            f"-L{os.path.join(torch_dir, 'lib')}", f"-L{PKG_DIR}",
            "-lnvfp4dg", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-           "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

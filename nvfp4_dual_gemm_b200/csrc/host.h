@@ -8,6 +8,8 @@
 
 #include <string>
 
+#include "nvfp4_dual_gemm.h"
+
 namespace nvfp4dg {
 
 // Device error word bits (role whose bounded wait expired).
@@ -41,5 +43,15 @@ int host_byte_map(const void* ptr, long long rows, long long row_bytes,
 
 // NVFP4DG_FLAG_SYNC_CHECK: waits for `stream` and reads the error word.
 int host_sync_check(cudaStream_t stream);
+
+// Runs a C entry point's body: no C++ exception leaves it.
+template <typename F>
+int host_guarded(F body) {
+  try {
+    return body();
+  } catch (...) {
+    return NVFP4DG_ERR_CUDA;  // out of host memory
+  }
+}
 
 }  // namespace nvfp4dg

@@ -44,7 +44,6 @@ constexpr int kSfWarps = 4;
 constexpr int kEpiWarp1 = 11;
 constexpr int kTmemCols = 512;
 constexpr int kMaxStages = 8;
-constexpr int kMaxSplit = 8;
 constexpr int kMaxGroups = 256;
 constexpr int kSmemBudget = 221 * 1024;  // dynamic; static holds the groups
 
@@ -1580,64 +1579,92 @@ struct LinearPlan {
   int split;   // CTAs that share a tile's K range
   int grid;    // CTAs
   int tiles;
-  int kblocks;
+  int kblocks;  // K blocks of a tile
 };
 
-// `mt`: token tiles of 32, 64, 128 and 256 tokens (of all groups).
-LinearPlan plan_linear(const long long (&mts)[4], int N, int K, int groups,
-                       unsigned flags, int sms) {
-  LinearPlan pl{};
-  const int n_tiles = (N + kFeat - 1) / kFeat;
-  const int kblocks = (K + 255) / 256;
-  const long long pair_tiles = mts[3] * ((N + 255) / 256);
+// What a launch takes, in microseconds, fitted to B200 timings of 1 to 2048
+// tokens (N 512 to 8192, K 1024 to 14336, graph-replayed, L2 warm): a start
+// and end, the first wave of tiles, and every further one, which is bound by
+// its products or by its epilogue.  `kb`: the 256-wide K blocks of a CTA.
+double linear_cost(int tn, double kb, double waves, bool split, int tokens,
+                   bool residual) {
+  if (tn == 32) {
+    const double wave = 0.20 * kb + 0.1;
+    return 3.5 + 0.03 * std::min(tokens, 32) + (split ? 0.25 : 0.0) + wave +
+           (waves - 1) * std::max(wave, 1.5);
+  }
+  if (tn == 64) {
+    const double wave = 0.24 * kb + 0.3;
+    return 5.0 + (split ? 0.7 : 0.0) + wave +
+           (waves - 1) * std::max(wave, 2.6);
+  }
+  if (tn == 128) {
+    const double wave = 0.40 * kb + 0.5;
+    return 5.0 + (split ? 0.2 : 0.0) + wave +
+           (waves - 1) * std::max(wave, 3.3);
+  }
+  return 3.5 + waves * (0.41 * kb + (residual ? 6.3 : 2.8));
+}
+
+// `mts`: token tiles of 32, 64, 128 and 256 tokens (of all groups); `tokens`:
+// of all of them.
+LinearPlan plan_linear(const long long (&mts)[4], long long tokens, int N,
+                       int K, int groups, bool residual, unsigned flags,
+                       int sms) {
   const unsigned forced_tile =
       flags & (NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
                NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR);
-  const long long units = sms / 2;
-  // waves of tiles, each by its K blocks' time
-  const double pair_cost =
-      double((pair_tiles + units - 1) / units) * (kblocks * 620.0 + 2500);
-  const double one_cost =
-      double((mts[2] * n_tiles + sms - 1) / sms) * (kblocks * 560.0 + 1500);
-  if (sms >= 2 && ((flags & NVFP4DG_LINEAR_PAIR) ||
-                   (!forced_tile && mts[2] > mts[3] && pair_cost < one_cost))) {
-    pl.tn = 256;
-    pl.split = 1;
-    pl.kblocks = kblocks;
-    pl.tiles = static_cast<int>(std::min<long long>(pair_tiles, 1 << 30));
-    pl.grid = 2 * static_cast<int>(std::min<long long>(pair_tiles, units));
-    return pl;
-  }
-  // the narrowest tile that holds as few tiles as the widest: columns beyond
-  // the tokens cost shared memory and MMA time
-  if (flags & NVFP4DG_LINEAR_TOKENS32)
-    pl.tn = 32;
-  else if (flags & NVFP4DG_LINEAR_TOKENS64)
-    pl.tn = 64;
-  else if (flags & NVFP4DG_LINEAR_TOKENS128)
-    pl.tn = 128;
-  else
-    pl.tn = mts[0] == mts[2] ? 32 : mts[1] == mts[2] ? 64 : 128;
-  const long long mt = pl.tn == 32 ? mts[0] : pl.tn == 64 ? mts[1] : mts[2];
-  pl.tiles = static_cast<int>(std::min<long long>(mt * n_tiles, 1 << 30));
-  pl.split = 1;
-  pl.kblocks = pl.tn <= 64 ? (K + 511) / 512 : kblocks;
-  const int forced =
+  const int forced_split =
       static_cast<int>((flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8);
-  if (groups == 0 && forced > 0) {
-    pl.split = 1 << (forced - 1);
-  } else if (groups == 0) {
-    for (int s = kMaxSplit; s > 1; s /= 2)
-      if ((long long)pl.tiles * s <= sms && kblocks >= 2 * s &&
-          pl.kblocks >= s) {
-        pl.split = s;
+  const int kb256 = (K + 255) / 256;
+  LinearPlan best{};
+  double best_cost = 1e300;
+  for (int i = 0; i < 4; ++i) {
+    if (forced_tile && !(forced_tile & (1u << i))) continue;
+    const int tn = 32 << i;
+    const int ctas = tn == 256 ? 2 : 1;
+    if (sms < ctas) continue;
+    LinearPlan pl{};
+    pl.tn = tn;
+    pl.kblocks = tn <= 64 ? (K + 511) / 512 : kb256;
+    const long long n_tiles =
+        tn == 256 ? (N + 255) / 256 : (N + kFeat - 1) / kFeat;
+    pl.tiles = static_cast<int>(std::min<long long>(mts[i] * n_tiles,
+                                                    1 << 30));
+    for (int lg = 0; lg < 4; ++lg) {
+      const int s = 1 << lg;
+      // the CTAs of a cluster share a tile's K range: one problem only, a
+      // block for each, and all clusters at once (a cluster lies in one
+      // group of SMs, which leaves some of them over)
+      const int room = s == 2 ? sms / 2 - 2 : s == 4 ? sms / 4 - 3
+                                            : sms / 8 - 4;
+      if (s > 1 && (groups > 0 || tn == 256 || s > pl.kblocks)) break;
+      if (forced_split && groups == 0 && tn < 256) {
+        const bool last = 2 * s > pl.kblocks || lg == 3;
+        if (lg + 1 != forced_split && !(last && lg + 1 < forced_split))
+          continue;
+      } else if (s > 1 && pl.tiles > room) {
         break;
       }
+      pl.split = s;
+      const long long units = sms / ctas;
+      const double waves =
+          s > 1 ? 1.0
+                : static_cast<double>((pl.tiles + units - 1) / units);
+      const double cost =
+          linear_cost(tn, static_cast<double>(kb256) / s, waves, s > 1,
+                      static_cast<int>(std::min<long long>(tokens, 32)),
+                      residual);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = pl;
+        best.grid = s > 1 ? pl.tiles * s
+                          : ctas * static_cast<int>(
+                                       std::min<long long>(pl.tiles, units));
+      }
+    }
   }
-  pl.split = std::min(pl.split, pl.kblocks);
-  while (pl.split & (pl.split - 1)) --pl.split;
-  pl.grid = pl.split > 1 ? pl.tiles * pl.split : std::min(pl.tiles, sms);
-  return pl;
+  return best;
 }
 
 template <typename T, int TN>
@@ -1742,6 +1769,8 @@ int check_linear(const nvfp4_linear_args* a, int groups,
                                  NVFP4DG_LINEAR_PAIR);
   if (t & (t - 1))
     return host_fail(NVFP4DG_ERR_INVALID, "the tile flags are exclusive");
+  if (a->alpha != a->alpha)
+    return host_fail(NVFP4DG_ERR_INVALID, "alpha is NaN");
   const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
                          NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR |
                          NVFP4DG_LINEAR_SPLIT_MASK |
@@ -1797,7 +1826,7 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
   LinearParams p;
   std::memset(&p, 0, sizeof(p));
-  long long mt[4] = {0, 0, 0, 0};
+  long long mt[4] = {0, 0, 0, 0}, tokens = 0;
   if (groups > 0 && !on_device) {
     long long next = 0;
     for (int g = 0; g < groups; ++g) {
@@ -1827,11 +1856,13 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
       mt[3] += (n + 255) / 256;
     }
     if (mt[0] == 0) return NVFP4DG_OK;
+    tokens = mt[0] * 32;
   } else {
-    // counts on the device: A's rows spread evenly, half a row block of each
-    // group taken for padding
+    // counts on the device: A's rows spread evenly, most of a row block of
+    // each group taken for padding
     long long per = groups ? (a->M + groups - 1) / groups : a->M;
-    if (groups) per = std::max(per - 64, (per + 1) / 2);
+    if (groups) per = std::max(per - 96, (per + 3) / 4);
+    tokens = per * std::max(groups, 1);
     const long long g = groups ? groups : 1;
     mt[0] = (per + 31) / 32 * g;
     mt[1] = (per + 63) / 64 * g;
@@ -1840,7 +1871,8 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   }
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
-  LinearPlan pl = plan_linear(mt, a->N, a->K, groups, a->flags, dev.sms);
+  LinearPlan pl = plan_linear(mt, tokens, a->N, a->K, groups,
+                              a->residual != nullptr, a->flags, dev.sms);
   // tiles counted by the kernel: a full grid
   if (groups > 0 && on_device)
     pl.grid = pl.tn == 256 ? dev.sms / 2 * 2 : dev.sms;
@@ -1911,37 +1943,48 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
 extern "C" {
 
 int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream) {
-  return nvfp4dg::run_linear(args, nullptr, nullptr, 0, false, stream);
+  return nvfp4dg::host_guarded([&] {
+    return nvfp4dg::run_linear(args, nullptr, nullptr, 0, false, stream);
+  });
 }
 
 int nvfp4_linear_run_grouped(const nvfp4_linear_args* args,
                              const int* group_rows, const int* group_row0,
                              int groups, int on_device, void* stream) {
-  nvfp4dg::host_clear_error();
-  if (groups < 1 || groups > nvfp4dg::kMaxGroups)
-    return nvfp4dg::host_fail(
-        NVFP4DG_ERR_INVALID,
-        "groups must be 1.." + std::to_string(nvfp4dg::kMaxGroups));
-  if (group_rows == nullptr)
-    return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID, "group_rows is required");
-  return nvfp4dg::run_linear(args, group_rows, group_row0, groups,
-                             on_device != 0, stream);
+  return nvfp4dg::host_guarded([&] {
+    nvfp4dg::host_clear_error();
+    if (groups < 1 || groups > nvfp4dg::kMaxGroups)
+      return nvfp4dg::host_fail(
+          NVFP4DG_ERR_INVALID,
+          "groups must be 1.." + std::to_string(nvfp4dg::kMaxGroups));
+    if (group_rows == nullptr)
+      return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
+                                "group_rows is required");
+    if (args != nullptr && args->residual != nullptr)
+      return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
+                                "grouped products take no residual");
+    return nvfp4dg::run_linear(args, group_rows, group_row0, groups,
+                               on_device != 0, stream);
+  });
 }
 
-int nvfp4_linear_plan(int M, int N, int K, unsigned flags, int num_sms,
-                      int* tokens_out, int* split_out, int* grid_out) {
-  nvfp4dg::host_clear_error();
-  if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 64 || num_sms <= 0)
-    return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
-                              "invalid problem for planning");
-  const long long mts[4] = {(M + 31ll) / 32, (M + 63ll) / 64,
-                            (M + 127ll) / 128, (M + 255ll) / 256};
-  const nvfp4dg::LinearPlan pl =
-      nvfp4dg::plan_linear(mts, N, K, 0, flags, num_sms);
-  if (tokens_out) *tokens_out = pl.tn;
-  if (split_out) *split_out = pl.split;
-  if (grid_out) *grid_out = pl.grid;
-  return NVFP4DG_OK;
+int nvfp4_linear_plan(int M, int N, int K, int residual, unsigned flags,
+                      int num_sms, int* tokens_out, int* split_out,
+                      int* grid_out) {
+  return nvfp4dg::host_guarded([&] {
+    nvfp4dg::host_clear_error();
+    if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 64 || num_sms <= 0)
+      return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
+                                "invalid problem for planning");
+    const long long mts[4] = {(M + 31ll) / 32, (M + 63ll) / 64,
+                              (M + 127ll) / 128, (M + 255ll) / 256};
+    const nvfp4dg::LinearPlan pl = nvfp4dg::plan_linear(
+        mts, M, N, K, 0, residual != 0, flags, num_sms);
+    if (tokens_out) *tokens_out = pl.tn;
+    if (split_out) *split_out = pl.split;
+    if (grid_out) *grid_out = pl.grid;
+    return NVFP4DG_OK;
+  });
 }
 
 }  // extern "C"

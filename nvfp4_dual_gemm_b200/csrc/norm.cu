@@ -833,12 +833,7 @@ int check_norm(const nvfp4_block_norm_args* a) {
   return NVFP4DG_OK;
 }
 
-}  // namespace
-}  // namespace nvfp4dg
-
-extern "C" int nvfp4_block_norm_run(const nvfp4_block_norm_args* a,
-                                    void* stream) {
-  using namespace nvfp4dg;
+int run_norm(const nvfp4_block_norm_args* a, void* stream) {
   host_clear_error();
   int rc = check_norm(a);
   if (rc || a->rows == 0) return rc;
@@ -858,4 +853,12 @@ extern "C" int nvfp4_block_norm_run(const nvfp4_block_norm_args* a,
   if (a->dtype == NVFP4DG_DTYPE_F16)
     return launch_norm<__half>(p, dev.sms, dev.id, s);
   return launch_norm<__nv_bfloat16>(p, dev.sms, dev.id, s);
+}
+
+}  // namespace
+}  // namespace nvfp4dg
+
+extern "C" int nvfp4_block_norm_run(const nvfp4_block_norm_args* a,
+                                    void* stream) {
+  return nvfp4dg::host_guarded([&] { return nvfp4dg::run_norm(a, stream); });
 }

@@ -13,6 +13,7 @@
 // ctypes call, which matters when a caller launches one call at a time.
 // Invalid arguments raise ValueError; CUDA and device failures RuntimeError.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
@@ -283,6 +284,12 @@ int64_t pitch(const at::Tensor& t) {
   return t.size(0) > 1 ? t.stride(0) : t.size(1);
 }
 
+// at::empty without its dispatch.
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType t,
+                      const at::Device& dev) {
+  return at::detail::empty_cuda(sizes, t, dev, c10::nullopt);
+}
+
 // What linear and linear_grouped share: everything but the groups.
 nvfp4_linear_args linear_args(const at::Tensor& A, const at::Tensor& B,
                               const at::Tensor& SFA, const at::Tensor& SFB,
@@ -388,7 +395,7 @@ at::Tensor linear(const at::Tensor& A, const at::Tensor& B,
     const at::ScalarType t = dtype.has_value()      ? *dtype
                              : residual.has_value() ? residual->scalar_type()
                                                     : at::kHalf;
-    C = at::empty({M, N}, A.options().dtype(t));
+    C = new_tensor({M, N}, t, A.device());
   }
   const nvfp4_linear_args a =
       linear_args(A, B, SFA, SFB, C, bias, activation, residual, row_scale,
@@ -585,7 +592,9 @@ NormOut norm(const at::Tensor& x_in, const OptTensor& y_in,
     y = same("y", *y_in);
     a.y = y.data_ptr();
     a.ldy = pitch(y);
-    out.R = R_in.has_value() ? *R_in : at::empty(x_in.sizes(), x.options());
+    out.R = R_in.has_value()
+                ? *R_in
+                : new_tensor(x_in.sizes(), x.scalar_type(), dev);
     r = same("R", out.R);
     a.R = r.data_ptr();
     a.ldr = pitch(r);
@@ -610,13 +619,14 @@ NormOut norm(const at::Tensor& x_in, const OptTensor& y_in,
   }
   if (pre && nvfp4) {
     if (Z_in.has_value()) bad("Z is for block_norm");
-    const auto u8 = x.options().dtype(at::kByte);
-    out.codes = at::empty({rows, D / 2}, u8);
-    out.sf = at::empty({blocked_bytes(rows, D)}, u8);
+    out.codes = new_tensor({rows, D / 2}, at::kByte, dev);
+    out.sf = new_tensor({blocked_bytes(rows, D)}, at::kByte, dev);
     a.codes = out.codes.data_ptr();
     a.sf = out.sf.data_ptr();
   } else if (pre) {
-    out.Z = Z_in.has_value() ? *Z_in : at::empty(x_in.sizes(), x.options());
+    out.Z = Z_in.has_value()
+                ? *Z_in
+                : new_tensor(x_in.sizes(), x.scalar_type(), dev);
     z = same("Z", out.Z);
     a.Z = z.data_ptr();
     a.ldz = pitch(z);
@@ -663,32 +673,10 @@ PYBIND11_MODULE(_C, m) {
   m.def("dual_gemm", &dual_gemm, py::arg("A"), py::arg("B1"), py::arg("B2"),
         py::arg("SFA"), py::arg("SFB1"), py::arg("SFB2"), py::arg("C"),
         py::arg("flags") = 0, py::arg("workspace") = py::none());
-  m.def("linear", &linear, py::arg("A"), py::arg("B"), py::arg("SFA"),
-        py::arg("SFB"), py::arg("C") = py::none(), py::kw_only(),
-        py::arg("bias") = py::none(), py::arg("activation") = py::none(),
-        py::arg("residual") = py::none(), py::arg("row_scale") = py::none(),
-        py::arg("alpha") = 1.0, py::arg("dtype") = py::none(),
-        py::arg("flags") = 0);
-  m.def("linear_grouped", &linear_grouped, py::arg("A"), py::arg("B"),
-        py::arg("SFA"), py::arg("SFB"), py::arg("C"), py::arg("group_rows"),
-        py::arg("group_row0") = py::none(), py::kw_only(),
-        py::arg("bias") = py::none(), py::arg("activation") = py::none(),
-        py::arg("row_scale") = py::none(), py::arg("alpha") = 1.0,
-        py::arg("flags") = 0);
-  m.def("block_norm", &block_norm, py::arg("x"), py::arg("y") = py::none(),
-        py::kw_only(), py::arg("weight") = py::none(),
-        py::arg("bias") = py::none(), py::arg("post_weight") = py::none(),
-        py::arg("post_bias") = py::none(), py::arg("gate") = py::none(),
-        py::arg("scale") = 1.0, py::arg("kind") = "rms",
-        py::arg("eps") = 1e-6, py::arg("post") = false,
-        py::arg("pre") = true, py::arg("R") = py::none(),
-        py::arg("Z") = py::none(), py::arg("flags") = 0);
-  m.def("block_norm_nvfp4", &block_norm_nvfp4, py::arg("x"),
-        py::arg("y") = py::none(), py::kw_only(),
-        py::arg("weight") = py::none(), py::arg("bias") = py::none(),
-        py::arg("post_weight") = py::none(),
-        py::arg("post_bias") = py::none(), py::arg("gate") = py::none(),
-        py::arg("scale") = 1.0, py::arg("kind") = "rms",
-        py::arg("eps") = 1e-6, py::arg("post") = false,
-        py::arg("R") = py::none(), py::arg("flags") = 0);
+  // (called with positional arguments: api.py holds the names and defaults,
+  // and keywords cost about a microsecond a call here)
+  m.def("linear", &linear);
+  m.def("linear_grouped", &linear_grouped);
+  m.def("block_norm", &block_norm);
+  m.def("block_norm_nvfp4", &block_norm_nvfp4);
 }

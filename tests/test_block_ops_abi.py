@@ -1,0 +1,160 @@
+"""CPU tests of the block operators' C ABI: every argument that must be
+refused is refused before anything touches a GPU, empty problems are no-ops,
+and the schedule of ``linear`` covers what it must."""
+import ctypes
+
+import pytest
+
+import nvfp4_dual_gemm_b200 as dg
+from nvfp4_dual_gemm_b200 import _lib
+
+P = 0x1000  # an aligned address that no refused call may follow
+
+
+def linear_args(**kw):
+    a = dict(A=P, B=P, SFA=P, SFB=P, C=P, ldc=256, M=4, N=256, K=128,
+             c_dtype=_lib.DTYPE_BF16, alpha=1.0)
+    a.update(kw)
+    return _lib.LinearArgs(**a)
+
+
+def run_linear(**kw):
+    return _lib.load().nvfp4_linear_run(ctypes.byref(linear_args(**kw)), None)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(M=-1), "non-negative"), (dict(N=252), "multiple of 8"),
+    (dict(K=96), "multiple of 64"), (dict(K=0), "multiple of 64"),
+    (dict(c_dtype=_lib.DTYPE_F32), "F16 or BF16"), (dict(c_dtype=9), "F16"),
+    (dict(bias=P, bias_dtype=_lib.DTYPE_F16), "bias"),
+    (dict(activation=5), "activation"), (dict(activation=-1), "activation"),
+    (dict(alpha=float("nan")), "alpha"),
+    (dict(flags=1 << 12), "flag"), (dict(flags=3), "exclusive"),
+    (dict(flags=0x500), "split"), (dict(C=None), "NULL"),
+    (dict(A=None), "NULL"), (dict(SFB=None), "NULL"),
+    (dict(ldc=248), "pitch"), (dict(residual=P, ldr=0), "pitch"),
+    (dict(ldc=1 << 23), "pitch"), (dict(M=(1 << 30) + 1), "too"),
+    (dict(M=1 << 30, N=1 << 20, ldc=1 << 20), "tiles"),
+])
+def test_linear_refuses(kw, word):
+    assert run_linear(**kw) == _lib.ERR_INVALID
+    assert word in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(A=P + 8), dict(SFA=P + 4), dict(C=P + 2), dict(ldc=260),
+    dict(residual=P + 8, ldr=256), dict(residual=P, ldr=262),
+    dict(bias=P + 2, bias_dtype=_lib.DTYPE_F32), dict(row_scale=P + 2),
+])
+def test_linear_refuses_misaligned(kw):
+    assert run_linear(**kw) == _lib.ERR_ALIGN
+
+
+def test_empty_problems_touch_nothing():
+    lib = _lib.load()
+    assert run_linear(M=0, A=None, C=None) == _lib.OK
+    assert run_linear(N=0, B=None, C=None) == _lib.OK
+    assert lib.nvfp4_linear_run(None, None) == _lib.ERR_INVALID
+    a = norm_args(rows=0, x=None)
+    assert lib.nvfp4_block_norm_run(ctypes.byref(a), None) == _lib.OK
+    # r is x and nothing else is asked for
+    a = norm_args(Z=None)
+    assert lib.nvfp4_block_norm_run(ctypes.byref(a), None) == _lib.OK
+
+
+def run_grouped(rows, row0=None, groups=None, **kw):
+    g = len(rows) if groups is None else groups
+    r = (ctypes.c_int * max(len(rows), 1))(*rows)
+    o = None if row0 is None else (ctypes.c_int * len(row0))(*row0)
+    return _lib.load().nvfp4_linear_run_grouped(
+        ctypes.byref(linear_args(**{"M": 512, **kw})), r, o, g, 0, None)
+
+
+@pytest.mark.parametrize("rows,row0,word", [
+    ([-1, 3], None, ">= 0"), ([3, 4], [0, 64], "128"),
+    ([3, 4], [-128, 128], "128"), ([130, 4], [0, 128], "overlaps"),
+    ([4, 4], [128, 0], "overlaps"), ([513], None, "past"),
+    ([1, 1, 1, 1, 1], None, "past"), ([4, 129], [0, 384], "past"),
+])
+def test_linear_grouped_refuses_host_groups(rows, row0, word):
+    assert run_grouped(rows, row0) == _lib.ERR_INVALID
+    assert word in _lib.last_error()
+
+
+def test_linear_grouped_refuses_counts_of_groups_and_residual():
+    assert run_grouped([1], groups=0) == _lib.ERR_INVALID
+    assert run_grouped([1] * 257) == _lib.ERR_INVALID
+    assert "256" in _lib.last_error()
+    assert run_grouped([1], residual=P, ldr=256) == _lib.ERR_INVALID
+    assert run_grouped([0, 0]) == _lib.OK  # every group empty
+    lib = _lib.load()
+    assert lib.nvfp4_linear_run_grouped(ctypes.byref(linear_args()), None,
+                                        None, 1, 1, None) == _lib.ERR_INVALID
+
+
+def norm_args(**kw):
+    a = dict(x=P, Z=P, ldx=64, ldy=64, ldr=64, ldz=64, rows=4, D=64,
+             dtype=_lib.DTYPE_BF16, eps=1e-6, scale=1.0)
+    a.update(kw)
+    return _lib.BlockNormArgs(**a)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(rows=-1), "rows"), (dict(D=60), "D %"), (dict(D=0), "D %"),
+    (dict(D=32776), "32768"), (dict(dtype=7), "dtype"),
+    (dict(w_dtype=_lib.DTYPE_F16), "weights"), (dict(kind=2), "norm"),
+    (dict(eps=-1e-6), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(flags=1), "flag"), (dict(x=None), "x is NULL"),
+    (dict(y=P), "R is required"), (dict(post=1), "need y"),
+    (dict(gate=P, gate_rows=1), "need y"),
+    (dict(y=P, R=P, gate=P, gate_rows=3), "divide"),
+    (dict(y=P, R=P, gate=P, gate_rows=0), "divide"),
+    (dict(codes=P), "together"), (dict(sf=P), "together"),
+    (dict(D=72, ldx=72, ldz=72, codes=P, sf=P), "64"), (dict(ldx=56), "least"),
+])
+def test_block_norm_refuses(kw, word):
+    a = norm_args(**kw)
+    assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+        _lib.ERR_INVALID
+    assert word in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=P + 8), dict(Z=P + 2), dict(weight=P + 4), dict(ldx=68),
+    dict(y=P, R=P, ldr=65),
+])
+def test_block_norm_refuses_misaligned(kw):
+    a = norm_args(**kw)
+    assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+        _lib.ERR_ALIGN
+
+
+@pytest.mark.parametrize("sms", [2, 20, 132, 148])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 64), (1, 4096, 4096),
+                                   (16, 4096, 14336), (333, 1480, 1344),
+                                   (8192, 8192, 28672), (5, 72, 320)])
+def test_plan_is_launchable(m, n, k, sms):
+    for residual in (False, True):
+        pl = dg.linear_plan(m, n, k, residual, num_sms=sms)
+        assert pl["tokens"] in (32, 64, 128, 256)
+        assert pl["split"] in (1, 2, 4, 8)
+        block = 512 if pl["tokens"] <= 64 else 256
+        assert pl["split"] <= -(-k // block)  # a K block for every CTA
+        assert 1 <= pl["grid"] <= sms
+        assert pl["grid"] % pl["split"] == 0
+        if pl["tokens"] == 256:
+            assert pl["grid"] % 2 == 0 and pl["split"] == 1
+
+
+def test_plan_follows_the_flags():
+    for flag, tokens in ((_lib.LINEAR_TOKENS32, 32),
+                         (_lib.LINEAR_TOKENS64, 64),
+                         (_lib.LINEAR_TOKENS128, 128),
+                         (_lib.LINEAR_PAIR, 256)):
+        for split in (1, 2, 4, 8):
+            pl = dg.linear_plan(40, 256, 4096, False,
+                                flag | _lib.linear_split(split))
+            assert pl["tokens"] == tokens
+            assert pl["split"] == (1 if tokens == 256 else split)
+    with pytest.raises(ValueError):
+        dg.linear_plan(4, 12, 64)

@@ -151,6 +151,31 @@ def test_nvfp4_equals_the_quantiser(rows, d, dtype):
     assert torch.equal(sf, want[2])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,d,gates", [(301, 1088, 7), (903, 2048, 903),
+                                          (640, 4160, 0), (1201, 7168, 1),
+                                          (299, 8192, 299)])
+def test_many_wide_rows(rows, d, gates, kind, dtype):
+    """More rows than the CTAs of a launch, in pairs, the last one alone."""
+    t = problem(rows, d, dtype, rows, gates, layer_bias=kind == "layer")
+    r, z = dg.block_norm(**t, kind=kind, scale=0.25)
+    want, err = reference(t, r, kind, 0.25)
+    check(z, want, err, "Z")
+    r2, codes, sf = dg.block_norm_nvfp4(**t, kind=kind, scale=0.25)
+    quant = dg.quantize_nvfp4(z, plain=False)
+    assert torch.equal(r, r2)
+    assert torch.equal(codes, quant[0]) and torch.equal(sf, quant[2])
+    t["x"] = t["x"].clone()
+    dg.block_norm(**t, kind=kind, scale=0.25, R=t["x"], Z=z)
+    assert torch.equal(t["x"], r)
+    _, z = dg.block_norm(r, weight=t["weight"], bias=t["bias"], kind=kind)
+    want, err = norm64(r.double(), kind, t["weight"], t["bias"], 1e-6)
+    check(z, want, err, "pre only")
+    r, none = dg.block_norm(t["y"], r, post=True, pre=False, kind=kind)
+    assert none is None
+
+
 def test_nvfp4_special_values():
     """NaN and infinite elements, zero rows and huge ones: the same bytes as
     the quantiser gives for Z."""
