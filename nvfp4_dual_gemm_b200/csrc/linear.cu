@@ -7,11 +7,13 @@
 // A (activations, [M, K]) and B (weights, [N, K]) are NVFP4 with blocked
 // scales, as for the dual GEMM; C is fp16 or bf16.
 //
-// linear_kernel gives the 128 TMEM lanes to the weights' rows and the
-// accumulator's columns to the tokens (C^T = B A^T): with few tokens, which
-// is where the product is bound by reading B once, the column side shrinks
-// to 32 while every lane still works, and a stage of the operand ring is
-// nearly all weights.
+// Two kernels.  linear_kernel: one CTA a tile of 128 features and 32 or 64
+// tokens, the features on the TMEM lanes and the tokens on the accumulator's
+// columns (C^T = B A^T): with few tokens, which is where the product is bound
+// by reading B once, the column side shrinks while every lane still works, and
+// a stage of the operand ring is nearly all weights.  With 128 tokens the two
+// change places.  linear_pair_kernel: two SMs a tile of 256 tokens x 256
+// features, for many tokens, where the tensor cores' feed is the bound.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -192,9 +194,10 @@ __device__ __forceinline__ Tile locate(const LinearParams& p,
 }
 
 // Whether the phase has completed, without waiting.  A wait on a barrier takes
-// ~300 cycles even when its phase is already complete, so each role asks for
-// its next stage before it works on the present one and waits only when the
-// answer was no: without that a K block took ~750 cycles whatever its size.
+// ~300 cycles even when its phase is already complete, so each role of
+// linear_kernel asks for its next stage before it works on the present one and
+// waits only when the answer was no (16 x 128 x 14336, one CTA: 26.4 -> 24.7
+// us).
 __device__ __forceinline__ bool mbar_peek(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -310,7 +313,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
 // x / (1 + 2^t): two special-function operations, five instructions.  (The
 // reciprocal by Newton steps on the FMA pipe halves the former and doubles
 // the latter; the epilogue's few warps wait on instructions, not on that
-// pipe.)  For t > 127 the denominator is infinite and the quotient a zero.
+// pipe: 16 experts of 1500 rows with silu took 29.7 us this way, 31.9 that
+// way.)  For t > 127 the denominator is infinite and the quotient a zero.
 __device__ __forceinline__ float quotient(float x, float t) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -525,9 +529,10 @@ __device__ __forceinline__ void store_row8(const LinearParams& p, int x, int n,
 
 // A stage of linear_kernel's ring holds kSub blocks of 256 along K.  What a
 // stage costs beyond its bytes, a wait of ~300 cycles in each role and the MMA
-// thread's commit, made a 256-wide block take ~710 cycles; two of them at once
-// take less than twice the half (460 each).  With 128 tokens a stage is twice
-// as deep in bytes and one block wide.
+// thread's commit, made a 256-wide block take ~710 cycles whatever the tokens;
+// two of them at once take ~535 each (16 x 4096 x 14336: 10.6 -> 10.1 us, by
+// then bound by memory).  With 128 tokens a stage is deeper in bytes and one
+// block wide.
 template <int TN>
 struct Cfg {
   // 128 tokens: the tokens take the TMEM lanes and 128 features the columns,
@@ -570,6 +575,11 @@ struct Cfg {
 // split > 1: the CTAs of a cluster share one tile's K range.  Each sends the
 // fp32 partials of the other ranks' token columns into their shared memory
 // and finishes its own share, adding the partials in rank order.
+//
+// Bound by: reading B once (16 x 4096 x 14336, 33 MB: 10.1 us, 3.3 TB/s
+// including ~4 us of start, exchange and end that short products consist of;
+// 1 x 4096 x 4096: 5.7 us), and for several tiles a CTA by the chain of a K
+// block or by the epilogue's instructions, whichever is longer.
 template <typename T, int TN>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmW,
@@ -665,9 +675,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kProdWWarp || warp == kProdXWarp) {
     // ---------------------------------------------------------- producers
-    // They only copy: a thread's instructions on barriers and copies take
-    // ~105 cycles each, and with the arming of both barriers in this loop a K
-    // block took ~1000 cycles whatever its size.
+    // They only copy; the barriers' expected bytes come with the scale warps'
+    // arrivals.
     {
       const bool w_side = warp == kProdWWarp;
       // the 128 lanes' operand comes through the first producer
@@ -1106,6 +1115,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 // CTAs' tiles land on its `full` barriers.  A thread of the epilogue is a
 // token row; outputs leave through shared memory and TMA stores, 64 columns
 // at a time.
+//
+// Bound by the ring's latency: a stage's tiles land ~2100 cycles after it is
+// free, its MMAs take 512 and the hand-offs ~1000, so that five stages give a
+// block every ~740 cycles where the tensor cores need 512; then by power
+// (8192 x 8192 x 28672: 855 us, 4.5 PFLOP/s; 4096 x 4096 x 14336: 117 us, 4.1
+// PFLOP/s).  Of a tile's epilogue ~2700 cycles (6500 with a residual) are not
+// hidden behind the next tile: there is one accumulator.  Tried and slower:
+// sixteen epilogue warps that hold the whole accumulator in registers (freed
+// after 500 cycles, but 80 registers a thread and half-size store boxes: K of
+// 1792 to 4096 5 to 15 % slower), their outputs stored without boxes (experts
+// of K 2048 a third slower), and scales copied ahead of their stage (two waits
+// in the scale warps: no gain).
 // ---------------------------------------------------------------------------
 constexpr int kPairThreads = 512;
 constexpr int kPairWaiter = 15;   // see below

@@ -9,6 +9,11 @@
 // One pass: a row stays in registers between its one read of x and y and its
 // one write of r and z; the row sums go through the warps' shuffles and, for
 // rows wider than a warp holds, one word a warp in shared memory.
+//
+// Bound by memory for many wide rows (8192 x 7168 bf16, post and pre RMS norm:
+// 75 us, 6.3 TB/s, 0.96 of the measured copy bandwidth), by instructions for
+// narrower ones (10800 x 2056: 38 us, 4.7 TB/s; layer norms 52 us), by latency
+// for few (1 x 7168: 3.0 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -573,6 +578,9 @@ __global__ void __launch_bounds__(MAXT)
 // memory while it computes: the copies in flight do not depend on how many
 // warps wait in a row's sums.  A thread holds one vector of both rows, so that
 // each barrier serves two sums, and the norms' weights stay in its registers.
+// (8192 x 7168 bf16: one row a CTA without the ring 130 us, with it 112; fp32
+// pairs 98; two rows 85; their sums in one set of shuffles and no divisions
+// 75.  With the weights read from L1 for every row, 151.)
 constexpr int kPairRows = 2;
 
 template <typename T, bool LAYER, int MAXT, int CTAS>
