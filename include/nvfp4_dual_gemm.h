@@ -279,8 +279,8 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
  * [M, K/2], SFA, B [N, K/2] and SFB are laid out as for the dual GEMM (dense
  * rows; blocked scales padded to 128 rows).  M >= 0, N % 8 == 0, K a positive
  * multiple of 64.  C and residual are row-major with row pitches of `ldc` /
- * `ldr` elements (>= N, multiples of 8); residual may be C itself.  bias, row_scale
- * and residual may be NULL.  All pointers are device pointers; A, B, SFA,
+ * `ldr` elements (>= N, multiples of 8); residual may be C itself, else the
+ * two must not overlap.  bias, row_scale and residual may be NULL.  All pointers are device pointers; A, B, SFA,
  * SFB, C and residual 16-byte aligned.  No workspace is used.  The reference
  * has no such product: its one kernel ends with the gated activation
  * (nvfp4_dual_gemm.cu:126-193).
@@ -332,7 +332,8 @@ NVFP4DG_API int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream);
  * when it is NULL, each group starts at the next multiple of 128 after the
  * one before.  Groups may be empty; rows of no group are not written.
  *   on_device == 0: group_rows and group_row0 are host arrays, read during
- *     the call; wrong or overlapping ones are refused.
+ *     the call; first rows ascend, and wrong or overlapping groups are
+ *     refused.
  *   on_device != 0: both are device arrays, read by the kernel (a router's
  *     counts without a copy to the host; a captured call reads them at each
  *     replay).  A negative count is an empty group; a group whose first row
@@ -366,8 +367,9 @@ NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, int residual,
  * not written.  gate is [gate_rows, D] of the stream's type, row i of it for
  * the i-th of gate_rows equal runs of rows (1: one gate for all; rows: one
  * for each).  The stream x, y, R, Z have one type (F32, F16 or BF16) and
- * their own row pitches in elements (multiples of 8 and >= D; F32: of 4); R
- * may be x or y.  Weights and biases are F32 or of the stream's type
+ * their own row pitches in elements (multiples of 8 and >= D; F32: of 4).  R
+ * and Z may each be x or y, but must not overlap one another or the gate, nor
+ * x or y in part.  Weights and biases are F32 or of the stream's type
  * (w_dtype).  Outputs of z, either or none:
  *   Z              in the stream's type;
  *   codes and sf   NVFP4 for the next product: [rows, D/2] e2m1 codes and

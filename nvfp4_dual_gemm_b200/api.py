@@ -296,7 +296,7 @@ def linear(A, B, SFA, SFB, C=None, *, bias=None, activation=None,
     :func:`dual_gemm` (any M, N % 8 == 0, K a positive multiple of 64).
     ``activation`` is None, "relu", "silu", "gelu_tanh" or "gelu"; ``bias``
     [N] is float32 or of C's type, ``row_scale`` [M] float32, ``residual``
-    [M, N] of C's type (it may be C itself).  Without ``C``, a contiguous
+    [M, N] of C's type (it may be C itself, but not overlap it in part).  Without ``C``, a contiguous
     output of ``dtype`` (default: the residual's type, else float16) is
     allocated.  C and residual may have strided rows (pitches of multiples
     of 8 elements).  Sums and the epilogue are fp32, rounded once.  Uses no
@@ -320,7 +320,8 @@ def linear_grouped(A, B, SFA, SFB, C, group_rows, group_row0=None, *,
     tensors, which the kernel reads itself: a router's counts need no copy to
     the host, and a captured call reads them at each replay.  Without
     ``group_row0`` each group starts at the next multiple of 128
-    (:func:`group_offsets`).  Up to 256 groups, any of them empty; rows of no
+    (:func:`group_offsets`); with it, groups on the host come in the order of
+    their rows.  Up to 256 groups, any of them empty; rows of no
     group are not written.  Counts on the host are checked; on the device, a
     group that is out of place is empty and one that reaches past the rows of
     A or C is cut there (``nvfp4_linear_run_grouped``)."""
@@ -360,8 +361,9 @@ def block_norm(x, y=None, *, weight=None, bias=None, post_weight=None,
     ``post_bias``.  Weights and biases [D] are float32 or of x's type (one
     type for all).  ``gate`` [G, D] (or [D]) holds one gate for each of G
     equal runs of rows: 1 for a channel gate, the batch for one a sample, the
-    rows for one a row.  ``R`` and ``Z`` are allocated when not given; R may
-    be x or y.  [rows, D] tensors may have strided rows (16-byte pitches).
+    rows for one a row.  ``R`` and ``Z`` are allocated when not given; each
+    may be x or y itself, but not overlap them in part, nor the other or the
+    gate.  [rows, D] tensors may have strided rows (16-byte pitches).
     D % 8 == 0 up to 32768.  Inference only (``nvfp4_block_norm_run``)."""
     return _lib.ext().block_norm(x, y, weight, bias, post_weight, post_bias,
                                  gate, scale, kind, eps, post, pre, R, Z,

@@ -6,6 +6,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cstdint>
 #include <string>
 
 #include "nvfp4_dual_gemm.h"
@@ -43,6 +44,28 @@ int host_byte_map(const void* ptr, long long rows, long long row_bytes,
 
 // NVFP4DG_FLAG_SYNC_CHECK: waits for `stream` and reads the error word.
 int host_sync_check(cudaStream_t stream);
+
+// How two row-major matrices of `rows` rows of `bytes` bytes lie (pitches in
+// bytes; NULL overlaps nothing).  Of matrices with different pitches whose
+// ranges meet, no row is looked at: they count as overlapping.
+enum class Overlap { kNone, kSame, kPart };
+inline Overlap host_overlap(const void* p, long long p_pitch, const void* q,
+                            long long q_pitch, long long rows,
+                            long long bytes) {
+  if (p == nullptr || q == nullptr || rows < 1 || bytes < 1)
+    return Overlap::kNone;
+  const unsigned long long a = reinterpret_cast<uintptr_t>(p);
+  const unsigned long long b = reinterpret_cast<uintptr_t>(q);
+  if (a == b && (rows == 1 || p_pitch == q_pitch)) return Overlap::kSame;
+  const unsigned long long row = bytes, pitch = p_pitch;
+  if (a + (rows - 1) * p_pitch + row <= b || b + (rows - 1) * q_pitch + row <= a)
+    return Overlap::kNone;
+  if (p_pitch == q_pitch) {  // columns of one wider matrix?
+    const unsigned long long d = a < b ? (b - a) % pitch : (a - b) % pitch;
+    if (d >= row && pitch - d >= row) return Overlap::kNone;
+  }
+  return Overlap::kPart;
+}
 
 // Runs a C entry point's body: no C++ exception leaves it.
 template <typename F>

@@ -832,6 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       int it = 0;
       bool ok = true, ready = false;
+      griddep_wait();  // (the waits' limits count from here)
       for (int tile = first; ok && tile < total; tile += step, ++it) {
         const int a = it & 1;
         if (!mbar_wait(&acc_empty_bar[a], ((it >> 1) & 1) ^ 1u, p.err,
@@ -1419,6 +1420,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int stage = 0;
       uint32_t acc_phase = 0, block = 0;
       bool ok = true, any = false;
+      griddep_wait();  // (the waits' limits count from here)
       for (int tile = first; ok && tile < total; tile += step) {
         if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
                                kErrMma)) {
@@ -1476,6 +1478,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       int stage = 0;
       uint32_t phase = 0, block = 0;
       bool ok = true;
+      griddep_wait();
       for (int tile = first; ok && tile < total; tile += step) {
         for (int kb = 0; kb < p.kblocks; ++kb) {
           if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
@@ -1767,6 +1770,23 @@ int launch_pair(const LinearParams& kp, const LinearPlan& pl,
   return NVFP4DG_OK;
 }
 
+int check_linear_flags(unsigned flags) {
+  const unsigned t = flags & (NVFP4DG_LINEAR_TOKENS32 |
+                              NVFP4DG_LINEAR_TOKENS64 |
+                              NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR);
+  if (t & (t - 1))
+    return host_fail(NVFP4DG_ERR_INVALID, "the tile flags are exclusive");
+  const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
+                         NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR |
+                         NVFP4DG_LINEAR_SPLIT_MASK |
+                         NVFP4DG_FLAG_SYNC_CHECK | NVFP4DG_FLAG_NO_PDL;
+  if (flags & ~known)
+    return host_fail(NVFP4DG_ERR_INVALID, "unknown flag bits");
+  if (((flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8) > 4)
+    return host_fail(NVFP4DG_ERR_INVALID, "split must be 1, 2, 4 or 8");
+  return NVFP4DG_OK;
+}
+
 int check_linear(const nvfp4_linear_args* a, int groups,
                  bool placed_on_device) {
   if (a == nullptr) return host_fail(NVFP4DG_ERR_INVALID, "args is NULL");
@@ -1784,22 +1804,9 @@ int check_linear(const nvfp4_linear_args* a, int groups,
     return host_fail(NVFP4DG_ERR_INVALID, "bias must be F32 or of C's type");
   if (a->activation < NVFP4DG_ACT_NONE || a->activation > NVFP4DG_ACT_GELU)
     return host_fail(NVFP4DG_ERR_INVALID, "unknown activation");
-  const unsigned t = a->flags & (NVFP4DG_LINEAR_TOKENS32 |
-                                 NVFP4DG_LINEAR_TOKENS64 |
-                                 NVFP4DG_LINEAR_TOKENS128 |
-                                 NVFP4DG_LINEAR_PAIR);
-  if (t & (t - 1))
-    return host_fail(NVFP4DG_ERR_INVALID, "the tile flags are exclusive");
+  if (const int rc = check_linear_flags(a->flags)) return rc;
   if (a->alpha != a->alpha)
     return host_fail(NVFP4DG_ERR_INVALID, "alpha is NaN");
-  const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
-                         NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR |
-                         NVFP4DG_LINEAR_SPLIT_MASK |
-                         NVFP4DG_FLAG_SYNC_CHECK | NVFP4DG_FLAG_NO_PDL;
-  if (a->flags & ~known)
-    return host_fail(NVFP4DG_ERR_INVALID, "unknown flag bits");
-  if (((a->flags & NVFP4DG_LINEAR_SPLIT_MASK) >> 8) > 4)
-    return host_fail(NVFP4DG_ERR_INVALID, "split must be 1, 2, 4 or 8");
   if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
   // tile numbers are 32-bit; groups placed by the device may overlap, so each
   // of them counts as all rows
@@ -1835,6 +1842,12 @@ int check_linear(const nvfp4_linear_args* a, int groups,
       reinterpret_cast<uintptr_t>(a->row_scale) % 4)
     return host_fail(NVFP4DG_ERR_ALIGN,
                      "bias and row_scale must be aligned to their elements");
+  // each output is written by the thread that read its residual, and by no
+  // other: in place is safe, a shift is not
+  if (host_overlap(a->C, 2 * a->ldc, a->residual, 2 * a->ldr, a->M,
+                   2ll * a->N) == Overlap::kPart)
+    return host_fail(NVFP4DG_ERR_INVALID,
+                     "residual must be C itself or not overlap it");
   return NVFP4DG_OK;
 }
 
@@ -1894,6 +1907,8 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   if ((rc = host_device(&dev))) return rc;
   LinearPlan pl = plan_linear(mt, tokens, a->N, a->K, groups,
                               a->residual != nullptr, a->flags, dev.sms);
+  if (pl.tn == 0)
+    return host_fail(NVFP4DG_ERR_INVALID, "pairs need two SMs");
   // tiles counted by the kernel: a full grid
   if (groups > 0 && on_device)
     pl.grid = pl.tn == 256 ? dev.sms / 2 * 2 : dev.sms;
@@ -1997,10 +2012,13 @@ int nvfp4_linear_plan(int M, int N, int K, int residual, unsigned flags,
     if (M <= 0 || N <= 0 || K <= 0 || N % 8 || K % 64 || num_sms <= 0)
       return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID,
                                 "invalid problem for planning");
+    if (const int rc = nvfp4dg::check_linear_flags(flags)) return rc;
     const long long mts[4] = {(M + 31ll) / 32, (M + 63ll) / 64,
                               (M + 127ll) / 128, (M + 255ll) / 256};
     const nvfp4dg::LinearPlan pl = nvfp4dg::plan_linear(
         mts, M, N, K, 0, residual != 0, flags, num_sms);
+    if (pl.tn == 0)
+      return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID, "pairs need two SMs");
     if (tokens_out) *tokens_out = pl.tn;
     if (split_out) *split_out = pl.split;
     if (grid_out) *grid_out = pl.grid;

@@ -838,6 +838,33 @@ int check_norm(const nvfp4_block_norm_args* a) {
     if (reinterpret_cast<uintptr_t>(q) % 16)
       return host_fail(NVFP4DG_ERR_ALIGN,
                        "every pointer must be 16-byte aligned");
+  // a thread writes the elements of x and y that it has read, and no others:
+  // in place is safe, a shift is not
+  const long long e = a->dtype == NVFP4DG_DTYPE_F32 ? 4 : 2;
+  auto lie = [&](const void* p, long long ldp, const void* q, long long ldq) {
+    return host_overlap(p, ldp * e, q, ldq * e, a->rows, a->D * e);
+  };
+  void* const r = a->y != nullptr ? a->R : nullptr;
+  if (lie(r, a->ldr, a->Z, a->ldz) != Overlap::kNone)
+    return host_fail(NVFP4DG_ERR_INVALID, "R and Z must not overlap");
+  if (lie(r, a->ldr, a->x, a->ldx) == Overlap::kPart ||
+      lie(r, a->ldr, a->y, a->ldy) == Overlap::kPart ||
+      lie(a->Z, a->ldz, a->x, a->ldx) == Overlap::kPart ||
+      lie(a->Z, a->ldz, a->y, a->ldy) == Overlap::kPart)
+    return host_fail(NVFP4DG_ERR_INVALID,
+                     "R and Z must each be x or y themselves or overlap "
+                     "neither");
+  if (a->gate != nullptr) {
+    const uintptr_t g0 = reinterpret_cast<uintptr_t>(a->gate);
+    const uintptr_t g1 = g0 + static_cast<size_t>(a->gate_rows) * a->D * e;
+    auto meets = [&](const void* p, long long ld) {
+      const uintptr_t q = reinterpret_cast<uintptr_t>(p);
+      return p != nullptr &&
+             q < g1 && g0 < q + ((a->rows - 1) * ld + a->D) * e;
+    };
+    if (meets(r, a->ldr) || meets(a->Z, a->ldz))
+      return host_fail(NVFP4DG_ERR_INVALID, "gate must not overlap R or Z");
+  }
   return NVFP4DG_OK;
 }
 

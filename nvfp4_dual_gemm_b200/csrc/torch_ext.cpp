@@ -305,6 +305,8 @@ nvfp4_linear_args linear_args(const at::Tensor& A, const at::Tensor& B,
     bad("K = " + std::to_string(K) + " must be a positive multiple of 64");
   check_blocked("SFA", SFA, A.size(0), K, 1);
   check_blocked("SFB", SFB, N, K, L);
+  no_grad_input("SFA", SFA);
+  no_grad_input("SFB", SFB);
   on_device("B", B, dev);
   on_device("SFA", SFA, dev);
   on_device("SFB", SFB, dev);
@@ -367,6 +369,8 @@ void check_operands(const at::Tensor& A, const at::Tensor& B, int64_t L) {
   check_bytes("A", A);
   check_bytes("B", B);
   if (A.dim() < 2 || B.dim() < 2) bad("A and B must be [rows, K/2]");
+  no_grad_input("A", A);
+  no_grad_input("B", B);
   rows_dense("A", A, A.size(0), A.size(1), 1);
   if (batches(B) != L)
     bad("B holds " + std::to_string(batches(B)) + " matrices, expected " +

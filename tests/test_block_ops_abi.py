@@ -158,3 +158,43 @@ def test_plan_follows_the_flags():
             assert pl["split"] == (1 if tokens == 256 else split)
     with pytest.raises(ValueError):
         dg.linear_plan(4, 12, 64)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(residual=P + 16, ldr=256),            # shifted within the rows
+    dict(residual=P + 512, ldr=256),           # by a row
+    dict(residual=P + 2 * 3 * 256, ldr=256),   # the last row
+    dict(residual=P, ldr=264),                 # another pitch
+    dict(ldc=504, residual=P + 512, ldr=504),  # rows that meet in a gap of N-8
+    dict(ldc=1024, residual=P + 256, ldr=1024),
+])
+def test_linear_refuses_a_residual_that_overlaps_c_in_part(kw):
+    assert run_linear(**kw) == _lib.ERR_INVALID
+    assert "overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(Z=P + 16), "Z must each"), (dict(Z=P + 128), "Z must each"),
+    (dict(Z=P, ldz=128), "Z must each"),
+    (dict(x=P + 4096, y=P, R=P + 128, Z=None), "Z must each"),
+    (dict(x=P + 4096, y=P + 8192, R=P, Z=P), "one another"),
+    (dict(x=P + 4096, y=P + 8192, R=P, Z=P + 384), "one another"),
+    (dict(x=P, y=P + 8192, R=P, Z=None, gate=P + 384, gate_rows=1), "gate"),
+    (dict(x=P + 4096, y=P + 8192, R=P + 4096, Z=P, gate=P - 384,
+          gate_rows=4), "gate"),
+])
+def test_block_norm_refuses_outputs_that_overlap(kw, word):
+    a = norm_args(**kw)
+    assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+        _lib.ERR_INVALID
+    assert {"one another": "R and Z must not"}.get(word, word) in \
+        _lib.last_error()
+
+
+def test_plan_refuses_what_the_call_refuses():
+    for flags in (3, 0x500, 1 << 12):
+        with pytest.raises(ValueError):
+            dg.linear_plan(4, 128, 256, flags=flags)
+    with pytest.raises(ValueError):
+        dg.linear_plan(4, 128, 256, flags=_lib.LINEAR_PAIR, num_sms=1)
+    assert dg.linear_plan(4, 128, 256, num_sms=1)["grid"] == 1

@@ -245,3 +245,42 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, want)
+
+
+FIRST_IN_CAPTURE = """
+import torch
+import nvfp4_dual_gemm_b200 as dg
+x = torch.randn(5, 256, device="cuda").half()
+b = torch.randint(0, 256, (64, 128), dtype=torch.uint8, device="cuda")
+sfb = torch.full((128 * 16,), 0x30, dtype=torch.uint8, device="cuda")
+w = torch.ones(256, device="cuda")
+counts = torch.tensor([5], dtype=torch.int32, device="cuda")
+c2 = torch.zeros(5, 64, dtype=torch.float16, device="cuda")
+def step():
+    _, a, sfa = dg.block_norm_nvfp4(x, weight=w)
+    dg.linear_grouped(a, b, sfa, sfb, c2, counts)
+    return dg.linear(a, b, sfa, sfb)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c = step()
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, step()) and torch.equal(c, c2)
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import subprocess
+    import sys
+    out = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE],
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+def test_scales_that_ask_for_a_gradient_are_refused():
+    a, b, sfa, sfb = operands()
+    f8 = sfb.view(torch.float8_e4m3fn)
+    dg.linear(a, b, sfa, f8)
+    with pytest.raises(ValueError, match="inference only"):
+        dg.linear(a, b, sfa, f8.detach().requires_grad_())

@@ -221,3 +221,25 @@ def test_streams_and_graph():
     r2, z2 = dg.block_norm(r0, t["y"], weight=t["weight"])
     torch.cuda.synchronize()
     assert torch.equal(R, r2) and torch.equal(Z, z2)
+
+
+@pytest.mark.parametrize("rows,d", [(1, 7168), (40, 512), (800, 2048)])
+def test_every_in_place_form(rows, d):
+    t = problem(rows, d, torch.bfloat16, rows)
+    w = dict(weight=t["weight"], post_weight=t["post_weight"])
+    x, y = t["x"], t["y"]
+    r0, z0 = dg.block_norm(x, y, **w)
+    for r_at, z_at in (("x", "y"), ("y", "x"), ("x", None), (None, "x"),
+                       (None, "y")):
+        c = {"x": x.clone(), "y": y.clone(), None: None}
+        r, z = dg.block_norm(c["x"], c["y"], R=c[r_at], Z=c[z_at], **w)
+        assert torch.equal(r, r0) and torch.equal(z, z0)
+    z0 = dg.block_norm(x, weight=t["weight"])[1]
+    c = x.clone()
+    assert torch.equal(dg.block_norm(c, weight=t["weight"], Z=c)[1], z0)
+    with pytest.raises(ValueError):
+        dg.block_norm(x, y, R=c, Z=c)
+    wide = torch.zeros(rows + 1, d, dtype=x.dtype, device="cuda")
+    if rows > 1:
+        with pytest.raises(ValueError):
+            dg.block_norm(wide[1:], y, R=wide[:-1])

@@ -259,3 +259,26 @@ def test_grouped_replay_reads_new_counts():
         g.replay()
         torch.cuda.synchronize()
         p.check(new, dg.group_offsets(new))
+
+
+@pytest.mark.parametrize("tile", ["t32", "t128", "pair"])
+def test_residual_beside_c_in_one_matrix(tile):
+    """C and residual as the halves of one matrix, either way round."""
+    m, n, k = 300, 136, 320
+    rng = np.random.default_rng(5)
+    (a, sfa, _), (b, sfb, _) = (random_nvfp4(r, k, rng, 0x10, 0x24)
+                                for r in (m, n))
+    ops = (dev(a), dev(b), dev(blocked(sfa)), dev(blocked(sfb)))
+    flags = {"t32": _lib.LINEAR_TOKENS32, "t128": _lib.LINEAR_TOKENS128,
+             "pair": _lib.LINEAR_PAIR}[tile]
+    both = torch.randn(m, 2 * n, device="cuda").half()
+    halves = both[:, :n], both[:, n:]
+    for c, r in (halves, halves[::-1]):
+        keep = r.clone()
+        want = dg.linear(*ops, residual=keep, flags=flags)
+        got = dg.linear(*ops, c, residual=r, flags=flags)
+        assert torch.equal(got, want) and torch.equal(r, keep)
+    with pytest.raises(ValueError):
+        dg.linear(*ops, both[:-1, :n], residual=both[1:, :n], flags=flags)
+    with pytest.raises(ValueError):
+        dg.linear(*ops, both[:, :n], residual=both[:, 8:n + 8], flags=flags)
