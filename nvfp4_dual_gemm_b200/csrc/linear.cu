@@ -252,6 +252,16 @@ __device__ __forceinline__ void tc_commit_both(uint64_t* bar) {
       : "memory");
 }
 
+// A warpgroup's share of the registers (all four warps together).
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
@@ -481,6 +491,15 @@ __device__ __forceinline__ void load_residual_row(const LinearParams& p,
   }
 }
 
+// Elements 2i and 2i + 1.
+__device__ __forceinline__ F2 get2(const float (&v)[32], int i) {
+  return {v[2 * i], v[2 * i + 1]};
+}
+__device__ __forceinline__ void set2(float (&v)[32], int i, F2 x) {
+  v[2 * i] = x.x;
+  v[2 * i + 1] = x.y;
+}
+
 // `residual(q)` gives its eight elements from column 8 q, `emit(q, o)` takes
 // the outputs there.
 template <typename T, typename R, typename E>
@@ -488,18 +507,18 @@ __device__ __forceinline__ void finish_row32(const LinearParams& p,
                                              float scale, const float* bias,
                                              float (&v)[32], R residual,
                                              E emit) {
+  const F2 alpha = {p.alpha, p.alpha};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float4 b = reinterpret_cast<const float4*>(bias)[i];
-    v[4 * i + 0] = fmaf(p.alpha, v[4 * i + 0], b.x);
-    v[4 * i + 1] = fmaf(p.alpha, v[4 * i + 1], b.y);
-    v[4 * i + 2] = fmaf(p.alpha, v[4 * i + 2], b.z);
-    v[4 * i + 3] = fmaf(p.alpha, v[4 * i + 3], b.w);
+    set2(v, 2 * i, fma2(alpha, get2(v, 2 * i), {b.x, b.y}));
+    set2(v, 2 * i + 1, fma2(alpha, get2(v, 2 * i + 1), {b.z, b.w}));
   }
   activate<32>(v, p.act);
   if (p.row_scale != nullptr) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= scale;
+    for (int i = 0; i < 16; ++i)
+      set2(v, i, mul2(get2(v, i), {scale, scale}));
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -509,8 +528,7 @@ __device__ __forceinline__ void finish_row32(const LinearParams& p,
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = unpack2<T>(w[i]);
-        v[8 * q + 2 * i] += f.x;
-        v[8 * q + 2 * i + 1] += f.y;
+        set2(v, 4 * q + i, add2(get2(v, 4 * q + i), {f.x, f.y}));
       }
     }
     emit(q, make_uint4(pack2<T>(v[8 * q + 0], v[8 * q + 1]),
@@ -1120,17 +1138,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Bound by the ring's latency: a stage's tiles land ~2100 cycles after it is
 // free, its MMAs take 512 and the hand-offs ~1000, so that five stages give a
 // block every ~740 cycles where the tensor cores need 512; then by power
-// (8192 x 8192 x 28672: 855 us, 4.5 PFLOP/s; 4096 x 4096 x 14336: 117 us, 4.1
-// PFLOP/s).  Of a tile's epilogue ~2700 cycles (6500 with a residual) are not
-// hidden behind the next tile: there is one accumulator.  Tried and slower:
-// sixteen epilogue warps that hold the whole accumulator in registers (freed
-// after 500 cycles, but 80 registers a thread and half-size store boxes: K of
-// 1792 to 4096 5 to 15 % slower), their outputs stored without boxes (experts
-// of K 2048 a third slower), and scales copied ahead of their stage (two waits
-// in the scale warps: no gain).
+// (timed in turns with short pauses: 8192 x 8192 x 28672 768 us, 5.0 PFLOP/s;
+// 4096 x 4096 x 14336 with a residual 115 us, 4.2 PFLOP/s).  There is one
+// accumulator, and a tile's epilogue takes ~6000 cycles: so its 256 columns go
+// to registers at once and the next tile's products start under it (126 ->
+// 115 us and 781 -> 768 us for the two, 122 -> 114 us for 32 experts of 512
+// rows and K 2048; a tile whose rows are stored one by one is slower, 37 ->
+// 39 us for 16 experts of ~94 rows, which the schedule gives smaller tiles).
+// That needs 192 registers in the epilogue's threads and hence the warpgroups'
+// shares; a spilled register costs more than elsewhere, as shared memory
+// leaves next to no L1.  Tried and slower: sixteen epilogue warps with half the
+// columns each, outputs stored without boxes, the columns in four rounds
+// through 64 registers (122 -> 139 us), and scales copied ahead of their stage
+// (two waits in the scale warps: no gain).
 // ---------------------------------------------------------------------------
 constexpr int kPairThreads = 512;
-constexpr int kPairWaiter = 15;   // see below
+// Whole warpgroups, whose shares of the launch's registers follow their work:
+// epilogue group 0 (warps 0-3), producers, MMA issuer and waiter (4-7), scale
+// warps (8-11), epilogue group 1 (12-15).
+constexpr int kPairSfWarp0 = 8;
+constexpr int kPairEpiWarp1 = 12;
+constexpr int kPairRegs = 65536 / kPairThreads;  // a thread's at launch
+constexpr int kPairEpiRegs = 192, kPairIssueRegs = 56, kPairSfRegs = 72;
+static_assert(2 * kPairEpiRegs + kPairIssueRegs + kPairSfRegs <= 4 * kPairRegs,
+              "an increase beyond the launch's registers would never end");
 constexpr int kPairStages = 5;
 constexpr int kPairTile = 128 * kRowBytes;  // one CTA's token or weight rows
 constexpr int kPairStageBytes = 2 * kPairTile + 3 * kRunBytes;
@@ -1268,84 +1299,173 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int first = static_cast<int>(blockIdx.x) / 2;
   const int step = static_cast<int>(gridDim.x) / 2;
 
-  if (warp == kProdWWarp || warp == kProdXWarp) {
-    // ---------------------------------------------------------- producers
-    // Warp 4: token scales, the first run of weight scales, token rows; warp
-    // 5: the second run, weight rows.  They only copy: the expected bytes
-    // come with the scale warps' arrivals.
-    {
-      const bool x_side = warp == kProdWWarp;
-      const uint64_t pol = x_side ? kPolicyEvictLast : kPolicyEvictNormal;
-      const uint32_t full_c = mapa_shared(smem_u32(&full_bar[0]), 0);
-      int stage = 0;
-      uint32_t phase = 0;
-      long long issued = 0;
-      bool ok = true;
-      griddep_wait();  // global memory only after the previous grid
-      for (int tile = first; ok && tile < total; tile += step) {
-        const PairTile t = locate_pair(p, tab, tile);
-        const int row = (x_side ? t.x0 : t.n0) + 128 * static_cast<int>(rank);
-        // the odd CTA's rows may lie past the problem's last row block, and
-        // the second weight run past the last one: they copy the last, whose
-        // products are never stored
-        const uint8_t* sfa =
-            p.sfa + (size_t)min(t.x0 / 128 + static_cast<int>(rank),
-                                t.sfa_last) *
-                        kblk64 * kAtomBytes;
-        const int nb = t.n0 / 128 + (x_side ? 0 : 1);
-        const uint8_t* sfb = p.sfb + (size_t)t.g * p.sfb_group +
-                             (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
-                                 kAtomBytes;
-        for (int kb = 0; lane == 0 && kb < p.kblocks; ++kb) {
-          if (issued >= S &&
-              !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
-                                 kErrProducer)) {
+  if (warp >= kProdWWarp && warp < kPairSfWarp0) {
+    reg_dec<kPairIssueRegs>();
+    if (warp == kProdWWarp || warp == kProdXWarp) {
+      // ---------------------------------------------------------- producers
+      // Warp 4: token scales, the first run of weight scales, token rows; warp
+      // 5: the second run, weight rows.  They only copy: the expected bytes
+      // come with the scale warps' arrivals.
+      {
+        const bool x_side = warp == kProdWWarp;
+        const uint64_t pol = x_side ? kPolicyEvictLast : kPolicyEvictNormal;
+        const uint32_t full_c = mapa_shared(smem_u32(&full_bar[0]), 0);
+        int stage = 0;
+        uint32_t phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        griddep_wait();  // global memory only after the previous grid
+        for (int tile = first; ok && tile < total; tile += step) {
+          const PairTile t = locate_pair(p, tab, tile);
+          const int row = (x_side ? t.x0 : t.n0) + 128 * static_cast<int>(rank);
+          // the odd CTA's rows may lie past the problem's last row block, and
+          // the second weight run past the last one: they copy the last, whose
+          // products are never stored
+          const uint8_t* sfa =
+              p.sfa + (size_t)min(t.x0 / 128 + static_cast<int>(rank),
+                                  t.sfa_last) *
+                          kblk64 * kAtomBytes;
+          const int nb = t.n0 / 128 + (x_side ? 0 : 1);
+          const uint8_t* sfb = p.sfb + (size_t)t.g * p.sfb_group +
+                               (size_t)min(nb, (p.N - 1) / 128) * kblk64 *
+                                   kAtomBytes;
+          for (int kb = 0; lane == 0 && kb < p.kblocks; ++kb) {
+            if (issued >= S &&
+                !mbar_wait_cluster(&empty_bar[stage], phase ^ 1u, p.err,
+                                   kErrProducer)) {
+              ok = false;
+              break;
+            }
+            const int next = stage + 1 == S ? 0 : stage + 1;
+            const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
+            uint8_t* st = smem + stage * kPairStageBytes;
+            uint8_t* sf = st + 2 * kPairTile;
+            const size_t run =
+                (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes;
+            const uint32_t full_s = full_c + 8u * static_cast<uint32_t>(stage);
+            if (x_side) {
+              bulk_load(sf, sfa + run, run_bytes, &sfdata_bar[stage], pol);
+              bulk_load(sf + kRunBytes, sfb + run, run_bytes,
+                        &sfdata_bar[stage], pol);
+              tma_load_3d_pair(st, &tmX, full_s, kb * kRowBytes, row, 0, pol);
+            } else {
+              bulk_load(sf + 2 * kRunBytes, sfb + run, run_bytes,
+                        &sfdata_bar[stage], pol);
+              tma_load_3d_pair(st + kPairTile, &tmW, full_s, kb * kRowBytes,
+                               row, t.g, pol);
+            }
+            ++issued;
+            stage = next;
+            phase = next_phase;
+          }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+        }
+        const bool ok_all = ok;
+        // never leave with copies in flight: scale runs land on this CTA's
+        // barriers, both CTAs' tiles on the even one's
+        for (int s = 0; s < S; ++s) {
+          if (issued > s) {
+            const uint32_t par =
+                static_cast<uint32_t>(((issued - 1 - s) / S) & 1);
+            mbar_wait(&sfdata_bar[s], par, p.err, kErrDrain, false);
+            if (x_side && leader)
+              mbar_wait_cluster(&full_bar[s], par, p.err, kErrDrain, false);
+            // the stage's last commit, which the even CTA sends to both: none
+            // may be on its way when a CTA leaves
+            if (ok_all)
+              mbar_wait_cluster(&empty_bar[s], par, p.err, kErrDrain, false);
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------- MMA issuer
+      if (lane == 0 && leader) {
+        constexpr uint32_t kIdesc = idesc_nvf4(256, 256);
+        const uint64_t x_desc0 =
+            smem_desc(smem_u32(smem), 16, 1024, SmemLayout::kSwizzle128B);
+        const uint64_t w_desc0 = smem_desc(smem_u32(smem) + kPairTile, 16, 1024,
+                                           SmemLayout::kSwizzle128B);
+        int stage = 0;
+        uint32_t acc_phase = 0, block = 0;
+        bool ok = true, any = false;
+        griddep_wait();  // (the waits' limits count from here)
+        for (int tile = first; ok && tile < total; tile += step) {
+          if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
+                                 kErrMma)) {
             ok = false;
             break;
           }
-          const int next = stage + 1 == S ? 0 : stage + 1;
-          const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
-          uint8_t* st = smem + stage * kPairStageBytes;
-          uint8_t* sf = st + 2 * kPairTile;
-          const size_t run =
-              (size_t)min(4 * kb, max(0, kblk64 - 4)) * kAtomBytes;
-          const uint32_t full_s = full_c + 8u * static_cast<uint32_t>(stage);
-          if (x_side) {
-            bulk_load(sf, sfa + run, run_bytes, &sfdata_bar[stage], pol);
-            bulk_load(sf + kRunBytes, sfb + run, run_bytes,
-                      &sfdata_bar[stage], pol);
-            tma_load_3d_pair(st, &tmX, full_s, kb * kRowBytes, row, 0, pol);
-          } else {
-            bulk_load(sf + 2 * kRunBytes, sfb + run, run_bytes,
-                      &sfdata_bar[stage], pol);
-            tma_load_3d_pair(st + kPairTile, &tmW, full_s, kb * kRowBytes,
-                             row, t.g, pol);
+          tc_fence_after();
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            if (!flag_wait(&landed_sh, ++block, p.err, kErrMma)) {
+              ok = false;
+              break;
+            }
+            const int next = stage + 1 == S ? 0 : stage + 1;
+            tc_fence_after();
+            const uint32_t soff =
+                static_cast<uint32_t>(stage) * (kPairStageBytes >> 4);
+            const uint32_t sf_t = tmem + kPairSfBase + stage * kPairSfCols;
+            const uint32_t acc0 = kb > 0 ? 1u : 0u;
+            if (4 * kb + 4 <= kblk64) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
+                                 w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
+                                 sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
+            } else {
+              for (int j = 0; j < kblk64 - 4 * kb; ++j)
+                tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
+                                 w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
+                                 sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
+            }
+            tc_commit_both(&empty_bar[stage]);
+            any = true;
+            stage = next;
           }
-          ++issued;
-          stage = next;
-          phase = next_phase;
+          if (!ok) break;
+          tc_commit_both(&acc_full_bar);
+          acc_phase ^= 1u;
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        // the last release of the accumulator (the odd CTA's warps arrive here
+        // remotely) is awaited like the others, so that no arrival is in
+        // flight when the CTAs leave
+        if (ok && any)
+          mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err, kErrMma);
+        tc_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
+        mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
       }
-      const bool ok_all = ok;
-      // never leave with copies in flight: scale runs land on this CTA's
-      // barriers, both CTAs' tiles on the even one's
-      for (int s = 0; s < S; ++s) {
-        if (issued > s) {
-          const uint32_t par =
-              static_cast<uint32_t>(((issued - 1 - s) / S) & 1);
-          mbar_wait(&sfdata_bar[s], par, p.err, kErrDrain, false);
-          if (x_side && leader)
-            mbar_wait_cluster(&full_bar[s], par, p.err, kErrDrain, false);
-          // the stage's last commit, which the even CTA sends to both: none
-          // may be on its way when a CTA leaves
-          if (ok_all)
-            mbar_wait_cluster(&empty_bar[s], par, p.err, kErrDrain, false);
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- waiter
+      // Waits for each K block's barrier in the MMA thread's stead and counts
+      // the blocks in shared memory, where that thread reads the count in a few
+      // cycles: its own wait would keep the tensor cores idle for ~300 cycles a
+      // block of 512.
+      if (lane == 0 && leader) {
+        int stage = 0;
+        uint32_t phase = 0, block = 0;
+        bool ok = true;
+        griddep_wait();
+        for (int tile = first; ok && tile < total; tile += step) {
+          for (int kb = 0; kb < p.kblocks; ++kb) {
+            if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
+              ok = false;
+              break;
+            }
+            flag_set(&landed_sh, ++block);
+            if (++stage == S) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
         }
       }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp >= kSfWarp0 && warp < kEpiWarp1) {
+  } else if (warp >= kPairSfWarp0 && warp < kPairEpiWarp1) {
+    reg_dec<kPairSfRegs>();
     // ---------------------------------------------------------- scale warps
     const uint32_t q = static_cast<uint32_t>(warp % 4);
     const uint32_t t_lane = tmem + ((32u * q) << 16);
@@ -1364,7 +1484,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t next_phase = phase ^ (next == 0 ? 1u : 0u);
         // arm the stage's next fill: it cannot complete before all four
         // scale warps have passed this one
-        if (warp == kSfWarp0 && lane == 0)
+        if (warp == kPairSfWarp0 && lane == 0)
           mbar_arrive_expect_tx(&sfdata_bar[stage], 3 * run_bytes);
         const int skip = 4 * kb - min(4 * kb, max(0, kblk64 - 4));
         const uint32_t sf_s =
@@ -1400,7 +1520,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) {
           const uint32_t full_s = mapa_shared(smem_u32(&full_bar[stage]), 0);
-          if (leader && warp == kSfWarp0)
+          if (leader && warp == kPairSfWarp0)
             mbar_arrive_expect_tx_cluster(full_s, 4 * kPairTile);
           else
             mbar_arrive_cluster(full_s);
@@ -1409,96 +1529,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         phase = next_phase;
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && leader) {
-      constexpr uint32_t kIdesc = idesc_nvf4(256, 256);
-      const uint64_t x_desc0 =
-          smem_desc(smem_u32(smem), 16, 1024, SmemLayout::kSwizzle128B);
-      const uint64_t w_desc0 = smem_desc(smem_u32(smem) + kPairTile, 16, 1024,
-                                         SmemLayout::kSwizzle128B);
-      int stage = 0;
-      uint32_t acc_phase = 0, block = 0;
-      bool ok = true, any = false;
-      griddep_wait();  // (the waits' limits count from here)
-      for (int tile = first; ok && tile < total; tile += step) {
-        if (!mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err,
-                               kErrMma)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!flag_wait(&landed_sh, ++block, p.err, kErrMma)) {
-            ok = false;
-            break;
-          }
-          const int next = stage + 1 == S ? 0 : stage + 1;
-          tc_fence_after();
-          const uint32_t soff =
-              static_cast<uint32_t>(stage) * (kPairStageBytes >> 4);
-          const uint32_t sf_t = tmem + kPairSfBase + stage * kPairSfCols;
-          const uint32_t acc0 = kb > 0 ? 1u : 0u;
-          if (4 * kb + 4 <= kblk64) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
-                               w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
-                               sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
-          } else {
-            for (int j = 0; j < kblk64 - 4 * kb; ++j)
-              tc_mma_nvf4_pair(tmem, x_desc0 + soff + 2u * j,
-                               w_desc0 + soff + 2u * j, kIdesc, sf_t + 4 * j,
-                               sf_t + 16 + 8 * j, j > 0 ? 1u : acc0);
-          }
-          tc_commit_both(&empty_bar[stage]);
-          any = true;
-          stage = next;
-        }
-        if (!ok) break;
-        tc_commit_both(&acc_full_bar);
-        acc_phase ^= 1u;
-      }
-      // the last release of the accumulator (the odd CTA's warps arrive here
-      // remotely) is awaited like the others, so that no arrival is in
-      // flight when the CTAs leave
-      if (ok && any)
-        mbar_wait_cluster(&acc_empty_bar, acc_phase ^ 1u, p.err, kErrMma);
-      tc_commit_pair(mapa_shared(smem_u32(&drain_bar), 0));
-      mbar_wait(&drain_bar, 0, p.err, kErrDrain, /*bail_on_err=*/false);
-    }
-    __syncwarp();
-  } else if (warp == kPairWaiter) {
-    // ---------------------------------------------------------- waiter
-    // Waits for each K block's barrier in the MMA thread's stead and counts
-    // the blocks in shared memory, where that thread reads the count in a few
-    // cycles: its own wait would keep the tensor cores idle for ~300 cycles a
-    // block of 512.
-    if (lane == 0 && leader) {
-      int stage = 0;
-      uint32_t phase = 0, block = 0;
-      bool ok = true;
-      griddep_wait();
-      for (int tile = first; ok && tile < total; tile += step) {
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          if (!mbar_wait_cluster(&full_bar[stage], phase, p.err, kErrMma)) {
-            ok = false;
-            break;
-          }
-          flag_set(&landed_sh, ++block);
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-    }
-    __syncwarp();
   } else {
+    reg_inc<kPairEpiRegs>();
     // ---------------------------------------------------------- epilogue
-    // Each group of four warps finishes 128 of the tile's columns in two
-    // phases of 64, through a box of its own.
-    const int q4 = warp % 4, group = epi_group(warp);
+    // Each group of four warps finishes 128 of the tile's columns, 32 at a
+    // time, and stores them 64 at a time through a box of its own.
+    const int q4 = warp % 4, group = warp >= kPairEpiWarp1 ? 1 : 0;
     const int row = 32 * q4 + lane;
     const bool stores = row == 0;  // the thread that stores the group's box
     const uint32_t t_row = tmem + (static_cast<uint32_t>(q4 * 32) << 16);
@@ -1528,55 +1564,67 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // the four warps leave together: they meet at the barriers below
       if (!epi_all(group, got)) break;
       tc_fence_after();
+      // the group's 128 columns at once, so that the accumulator is free for
+      // the next tile after one round trip
+      float v[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        tc_ld_32cols(t_row + 128 * group + 32 * c, v[c]);
+      tc_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tie32(v[c]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty_c);
       // a group's last rows are stored row by row: a box would overwrite the
       // rows behind them
       const bool boxed = p.groups == 0 ? rows > 0 : rows >= 128;
 #pragma unroll 1
-      for (int ph = 0; ph < 2; ++ph) {
-        const int n = n0 + 64 * ph;
-        float v[2][32];
-        uint4 res[2][4];
-        load_residual_row<T>(p, x, n, live, res[0]);
-        load_residual_row<T>(p, x, n + 32, live, res[1]);
-        __syncwarp();
-        tc_ld_32cols(t_row + 128 * group + 64 * ph, v[0]);
-        tc_ld_32cols(t_row + 128 * group + 64 * ph + 32, v[1]);
-        tc_wait_ld();
-        tie32(v[0]);
-        tie32(v[1]);
-        if (ph == 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_empty_c);
-        }
-        if (n >= p.N) continue;
-        if (boxed) {
+      for (int c = 0; c < 4; ++c) {
+        const int n = n0 + 32 * c, half = c & 1;
+        if (n >= p.N) break;
+        uint4 res[2];
+        if (boxed && half == 0) {
           // the store before has read the box
           if (stores) bulk_wait_group_read0();
           epi_bar(group);
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          finish_row32<T>(
-              p, scale, bias + 64 * ph + 32 * h, v[h],
-              [&](int i) { return res[h][i]; },
-              [&](int i, const uint4& o) {
-                if (boxed)
-                  sts128(smem_u32(box + row * 128 +
-                                  (((4 * h + i) ^ (row & 7)) << 4)),
-                         o);
-                else if (live && n + 32 * h + 8 * i < p.N)
-                  store_row8<T>(p, x, n + 32 * h + 8 * i, o);
-              });
-        }
-        if (boxed) {
+        finish_row32<T>(
+            p, scale, bias + 32 * c, v[0], [&](int i) {
+              // two at a time: four would not fit the registers
+              if ((i & 1) == 0) {
+                const T* r = static_cast<const T*>(p.residual) +
+                             (size_t)x * p.ldr + n + 8 * i;
+                res[0] = res[1] = make_uint4(0u, 0u, 0u, 0u);
+                if (live && n + 8 * i < p.N)
+                  res[0] = *reinterpret_cast<const uint4*>(r);
+                if (live && n + 8 * i + 8 < p.N)
+                  res[1] = *reinterpret_cast<const uint4*>(r + 8);
+              }
+              return res[i & 1];
+            },
+            [&](int i, const uint4& o) {
+              if (boxed)
+                sts128(smem_u32(box + row * 128 +
+                                (((4 * half + i) ^ (row & 7)) << 4)),
+                       o);
+              else if (live && n + 8 * i < p.N)
+                store_row8<T>(p, x, n + 8 * i, o);
+            });
+        if (boxed && (half == 1 || n + 32 >= p.N)) {
           fence_proxy_async_smem();
           epi_bar(group);
           if (stores) {
-            tma_store_2d(&tmC, box, 2 * n,
+            tma_store_2d(&tmC, box, 2 * (n - 32 * half),
                          t.x0 + 128 * static_cast<int>(rank));
             bulk_commit_group();
           }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {  // the next chunk into v[0]
+          v[0][i] = v[1][i];
+          v[1][i] = v[2][i];
+          v[2][i] = v[3][i];
         }
       }
     }
@@ -1743,7 +1791,15 @@ int launch_pair(const LinearParams& kp, const LinearPlan& pl,
   auto kernel = linear_pair_kernel<T>;
   const unsigned long long bit = 1ull << (dev & 63);
   if (!(ready.load() & bit)) {
-    cudaError_t e = cudaFuncSetAttribute(
+    cudaFuncAttributes fa;
+    cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
+    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncGetAttributes");
+    // the warpgroups' shares come out of what the launch allocates
+    if (fa.numRegs != kPairRegs)
+      return host_fail(NVFP4DG_ERR_CUDA,
+                       "linear_pair_kernel was built with " +
+                           std::to_string(fa.numRegs) + " registers");
+    e = cudaFuncSetAttribute(
         kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
     ready.fetch_or(bit);
