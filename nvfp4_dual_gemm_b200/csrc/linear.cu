@@ -1654,15 +1654,18 @@ struct LinearPlan {
   int kblocks;  // K blocks of a tile
 };
 
-// What a launch takes, in microseconds, fitted to B200 timings of 1 to 2048
-// tokens (N 512 to 8192, K 1024 to 14336, graph-replayed, L2 warm): a start
-// and end, the first wave of tiles, and every further one, which is bound by
-// its products or by its epilogue.  `kb`: the 256-wide K blocks of a CTA.
+// What a launch takes, in microseconds, fitted to B200 timings of 1 to 4000
+// tokens (N 512 to 8192, K 512 to 14336, graph-replayed, L2 warm): a start and
+// end, the first wave of tiles, and every further one, which is bound by its
+// products or by its epilogue.  `kb`: the 256-wide K blocks of a CTA;
+// `tokens`: 0 for groups, whose tiles say it all.  (500 x 8192 x 512: 8.2 us
+// with 128 tokens, 10.2 with pairs; x 7168: 27.0 and 20.1.)
 double linear_cost(int tn, double kb, double waves, bool split, int tokens,
                    bool residual) {
   if (tn == 32) {
     const double wave = 0.20 * kb + 0.1;
-    return 3.5 + 0.03 * std::min(tokens, 32) + (split ? 0.25 : 0.0) + wave +
+    return 3.5 + 0.03 * (tokens ? std::min(tokens, 32) : 32) +
+           (tokens > 64 ? 0.9 : 0.0) + (split ? 0.25 : 0.0) + wave +
            (waves - 1) * std::max(wave, 1.5);
   }
   if (tn == 64) {
@@ -1673,9 +1676,12 @@ double linear_cost(int tn, double kb, double waves, bool split, int tokens,
   if (tn == 128) {
     const double wave = 0.40 * kb + 0.5;
     return 5.0 + (split ? 0.2 : 0.0) + wave +
-           (waves - 1) * std::max(wave, 3.3);
+           (waves - 1) * (residual ? std::max(wave + 0.9, 4.0)
+                                   : std::max(wave, 2.4));
   }
-  return 3.5 + waves * (0.41 * kb + (residual ? 6.3 : 2.8));
+  return (residual ? 10.8 : 8.4) + 0.39 * kb +
+         (waves - 1) * (residual ? std::max(0.42 * kb + 2.5, 9.0)
+                                 : std::max(0.42 * kb + 1.0, 5.0));
 }
 
 // `mts`: token tiles of 32, 64, 128 and 256 tokens (of all groups); `tokens`:
@@ -1725,7 +1731,7 @@ LinearPlan plan_linear(const long long (&mts)[4], long long tokens, int N,
                 : static_cast<double>((pl.tiles + units - 1) / units);
       const double cost =
           linear_cost(tn, static_cast<double>(kb256) / s, waves, s > 1,
-                      static_cast<int>(std::min<long long>(tokens, 32)),
+                      groups ? 0 : static_cast<int>(tokens),
                       residual);
       if (cost < best_cost) {
         best_cost = cost;
