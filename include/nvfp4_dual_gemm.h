@@ -333,7 +333,7 @@ NVFP4DG_API int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream);
  * one before.  Groups may be empty; rows of no group are not written.
  *   on_device == 0: group_rows and group_row0 are host arrays, read during
  *     the call; first rows ascend, and wrong or overlapping groups are
- *     refused.
+ *     refused (whatever M and N are).
  *   on_device != 0: both are device arrays, read by the kernel (a router's
  *     counts without a copy to the host; a captured call reads them at each
  *     replay).  A negative count is an empty group; a group whose first row

@@ -1941,7 +1941,6 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   host_clear_error();
   int rc = check_linear(a, groups, on_device && group_row0 != nullptr);
   if (rc) return rc;
-  if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
   LinearParams p;
   std::memset(&p, 0, sizeof(p));
   long long mt[4] = {0, 0, 0, 0}, tokens = 0;
@@ -1973,9 +1972,10 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
       mt[2] += (n + 127) / 128;
       mt[3] += (n + 255) / 256;
     }
-    if (mt[0] == 0) return NVFP4DG_OK;
+    if (mt[0] == 0 || a->N == 0) return NVFP4DG_OK;
     tokens = mt[0] * 32;
   } else {
+    if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
     // counts on the device: A's rows spread evenly, most of a row block of
     // each group taken for padding
     long long per = groups ? (a->M + groups - 1) / groups : a->M;

@@ -198,3 +198,23 @@ def test_plan_refuses_what_the_call_refuses():
     with pytest.raises(ValueError):
         dg.linear_plan(4, 128, 256, flags=_lib.LINEAR_PAIR, num_sms=1)
     assert dg.linear_plan(4, 128, 256, num_sms=1)["grid"] == 1
+
+
+@pytest.mark.parametrize("rows,row0,word", [
+    ([-1], None, ">= 0"), ([5], [64], "128"), ([5], [-128], "128"),
+    ([130, 4], [0, 128], "overlaps"), ([513], None, "past"),
+])
+def test_empty_grouped_problems_check_their_groups(rows, row0, word):
+    assert run_grouped(rows, row0, N=0, B=None, C=None) == _lib.ERR_INVALID
+    assert word in _lib.last_error()
+    # (without rows of A, a group's reach past them comes before its overlap)
+    assert run_grouped(rows, row0, M=0, A=None, C=None) == _lib.ERR_INVALID
+    assert word in _lib.last_error() or "past" in _lib.last_error()
+
+
+def test_grouped_rows_need_rows_of_a():
+    empty = dict(M=0, A=None, C=None)
+    assert run_grouped([5], **empty) == _lib.ERR_INVALID
+    assert "past" in _lib.last_error()
+    assert run_grouped([0, 0], [0, 0], **empty) == _lib.OK
+    assert run_grouped([5], N=0, B=None, C=None) == _lib.OK
