@@ -416,7 +416,12 @@ std::vector<int> host_ints(const char* name, const py::object& o) {
   std::vector<int> v;
   const py::object seq = py::hasattr(o, "tolist") ? o.attr("tolist")() : o;
   for (const py::handle h : seq) {
-    const int64_t x = py::cast<int64_t>(h);
+    int64_t x;
+    try {
+      x = py::cast<int64_t>(h);
+    } catch (const py::cast_error&) {
+      bad(std::string(name) + " must hold integers of 32 bits");
+    }
     if (x < INT32_MIN || x > INT32_MAX)
       bad(std::string(name) + " does not fit 32 bits");
     v.push_back(static_cast<int>(x));

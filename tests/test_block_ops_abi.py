@@ -4,6 +4,7 @@ and the schedule of ``linear`` covers what it must."""
 import ctypes
 
 import pytest
+import torch
 
 import nvfp4_dual_gemm_b200 as dg
 from nvfp4_dual_gemm_b200 import _lib
@@ -218,3 +219,15 @@ def test_grouped_rows_need_rows_of_a():
     assert "past" in _lib.last_error()
     assert run_grouped([0, 0], [0, 0], **empty) == _lib.OK
     assert run_grouped([5], N=0, B=None, C=None) == _lib.OK
+
+
+@pytest.mark.parametrize("counts", [
+    [1.5], ["1"], "12", [2 ** 70], [2 ** 31], [[1, 2]], [None],
+    torch.tensor([1.5]), torch.tensor([[1, 2]]),
+])
+def test_counts_that_are_no_integers_are_refused(counts):
+    t = torch.zeros(4, 64, dtype=torch.uint8)
+    for kw in (dict(group_rows=counts),
+               dict(group_rows=[1], group_row0=counts)):
+        with pytest.raises(ValueError, match="group_row.*32 bits"):
+            dg.linear_grouped(t, t, t, t, t, **kw)
