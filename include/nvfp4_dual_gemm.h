@@ -280,8 +280,9 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
  * rows; blocked scales padded to 128 rows).  M >= 0, N % 8 == 0, K a positive
  * multiple of 64.  C and residual are row-major with row pitches of `ldc` /
  * `ldr` elements (>= N, multiples of 8); residual may be C itself, else the
- * two must not overlap.  bias, row_scale and residual may be NULL.  All pointers are device pointers; A, B, SFA,
- * SFB, C and residual 16-byte aligned.  No workspace is used.  The reference
+ * two must not overlap; C overlaps no other input.  bias, row_scale and
+ * residual may be NULL.  All pointers are device pointers; A, B, SFA, SFB, C
+ * and residual 16-byte aligned.  No workspace is used.  The reference
  * has no such product: its one kernel ends with the gated activation
  * (nvfp4_dual_gemm.cu:126-193).
  */

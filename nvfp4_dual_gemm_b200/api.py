@@ -296,10 +296,10 @@ def linear(A, B, SFA, SFB, C=None, *, bias=None, activation=None,
     :func:`dual_gemm` (any M, N % 8 == 0, K a positive multiple of 64).
     ``activation`` is None, "relu", "silu", "gelu_tanh" or "gelu"; ``bias``
     [N] is float32 or of C's type, ``row_scale`` [M] float32, ``residual``
-    [M, N] of C's type (it may be C itself, but not overlap it in part).  Without ``C``, a contiguous
-    output of ``dtype`` (default: the residual's type, else float16) is
-    allocated.  C and residual may have strided rows (pitches of multiples
-    of 8 elements).  Sums and the epilogue are fp32, rounded once.  Uses no
+    [M, N] of C's type (it may be C itself, but not overlap it in part; C
+    overlaps no other input).  Without ``C``, a contiguous output of ``dtype``
+    (default: the residual's type, else float16) is allocated.  C and residual
+    may have strided rows (pitches of multiples of 8 elements).  Sums and the epilogue are fp32, rounded once.  Uses no
     workspace and can be captured into a CUDA graph; inference only
     (``nvfp4_linear_run``).  For one token up to a few the CTAs of a cluster
     share each tile's K range; the result does not depend on timing."""

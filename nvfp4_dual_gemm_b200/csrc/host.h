@@ -67,6 +67,22 @@ inline Overlap host_overlap(const void* p, long long p_pitch, const void* q,
   return Overlap::kPart;
 }
 
+// Whether the `bytes` bytes from p meet a row of the matrix m.
+inline bool host_meets(const void* p, long long bytes, const void* m,
+                       long long pitch, long long rows, long long row) {
+  if (p == nullptr || m == nullptr || bytes < 1 || rows < 1 || row < 1)
+    return false;
+  const unsigned long long a = reinterpret_cast<uintptr_t>(p);
+  const unsigned long long b = reinterpret_cast<uintptr_t>(m);
+  const unsigned long long total = (rows - 1) * pitch + row;
+  if (a >= b + total || a + bytes <= b) return false;
+  if (rows == 1 || a < b) return true;
+  const unsigned long long in = (a - b) % pitch;  // from its row's start
+  return in < static_cast<unsigned long long>(row) ||
+         (in + bytes > static_cast<unsigned long long>(pitch) &&
+          a - b - in + pitch < total);
+}
+
 // Runs a C entry point's body: no C++ exception leaves it.
 template <typename F>
 int host_guarded(F body) {

@@ -1935,6 +1935,29 @@ int check_linear(const nvfp4_linear_args* a, int groups,
   return NVFP4DG_OK;
 }
 
+// CTAs read the inputs while others write C.
+int check_linear_overlap(const nvfp4_linear_args* a, int groups) {
+  const long long n = a->N, k = a->K, per = std::max(groups, 1);
+  const long long bias = a->bias_dtype == NVFP4DG_DTYPE_F32 ? 4 : 2;
+  const struct {
+    const char* name;
+    const void* p;
+    long long bytes;
+  } inputs[] = {
+      {"A", a->A, a->M * (k / 2)},
+      {"B", a->B, per * n * (k / 2)},
+      {"SFA", a->SFA, (a->M + 127ll) / 128 * (k / 64) * kAtomBytes},
+      {"SFB", a->SFB, per * ((n + 127) / 128) * (k / 64) * kAtomBytes},
+      {"bias", a->bias, per * n * bias},
+      {"row_scale", a->row_scale, a->M * 4ll},
+  };
+  for (const auto& in : inputs)
+    if (host_meets(in.p, in.bytes, a->C, 2 * a->ldc, a->M, 2 * n))
+      return host_fail(NVFP4DG_ERR_INVALID,
+                       std::string("C must not overlap ") + in.name);
+  return NVFP4DG_OK;
+}
+
 int run_linear(const nvfp4_linear_args* a, const int* group_rows,
                const int* group_row0, int groups, bool on_device,
                void* stream_ptr) {
@@ -1987,6 +2010,7 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
     mt[2] = (per + 127) / 128 * g;
     mt[3] = (per + 255) / 256 * g;
   }
+  if ((rc = check_linear_overlap(a, groups))) return rc;
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
   LinearPlan pl = plan_linear(mt, tokens, a->N, a->K, groups,

@@ -231,3 +231,33 @@ def test_counts_that_are_no_integers_are_refused(counts):
                dict(group_rows=[1], group_row0=counts)):
         with pytest.raises(ValueError, match="group_row.*32 bits"):
             dg.linear_grouped(t, t, t, t, t, **kw)
+
+
+FAR = 1 << 20  # apart from every other operand of these tests
+
+
+@pytest.mark.parametrize("where", [0, 512, 3 * 512 + 496, -16])
+@pytest.mark.parametrize("name", ["A", "B", "SFA", "SFB", "bias",
+                                  "row_scale"])
+def test_linear_refuses_a_c_that_meets_its_inputs(name, where):
+    c = 16 * FAR
+    kw = dict(A=FAR, B=2 * FAR, SFA=3 * FAR, SFB=4 * FAR, bias=5 * FAR,
+              row_scale=6 * FAR, C=c)
+    kw[name] = c + where
+    if name == "row_scale" and where < 0:
+        kw[name] = c - 4  # its last row
+    if name == "bias" and where == 0:
+        kw.update(bias=c - 4, bias_dtype=_lib.DTYPE_F32)
+    assert run_linear(**kw) == _lib.ERR_INVALID
+    assert "C must not overlap " + name in _lib.last_error()
+
+
+def test_linear_grouped_refuses_a_c_that_meets_a_later_groups_weights():
+    c = 16 * FAR
+    kw = dict(A=FAR, B=2 * FAR, SFA=3 * FAR, SFB=4 * FAR, bias=5 * FAR, C=c)
+    for name, size in (("B", 256 * 64), ("SFB", 2 * 2 * 512),
+                       ("bias", 256 * 4)):
+        # two groups: the second one's last 16 bytes are C's first
+        a = {**kw, name: c + 16 - 2 * size}
+        assert run_grouped([1, 1], **a) == _lib.ERR_INVALID
+        assert "C must not overlap " + name in _lib.last_error()

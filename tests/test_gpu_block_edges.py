@@ -1,0 +1,38 @@
+"""GPU tests of what the block operators' documentation allows at its edges:
+outputs beside their inputs in one buffer, tensors that autograd knows,
+schedules where a CTA's tiles belong to several groups, and many wide rows."""
+import pytest
+import torch
+
+import nvfp4_dual_gemm_b200 as dg
+
+pytestmark = pytest.mark.gpu
+
+
+def linear_operands(m, n, k, seed=0):
+    """Random codes and scales of 0.25 to 0.5 for A [m, k] and B [n, k]."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    u8 = dict(dtype=torch.uint8, device="cuda")
+
+    def matrix(rows):
+        return (torch.randint(0, 256, (rows, k // 2), generator=g, **u8),
+                torch.randint(0x28, 0x30, ((rows + 127) // 128 * 8 * k,),
+                              generator=g, **u8))
+    (a, sfa), (b, sfb) = matrix(m), matrix(n)
+    return a, b, sfa, sfb
+
+
+def test_c_beside_the_bias_in_one_buffer():
+    """The bias in the columns that a strided C leaves out is no overlap; in
+    C's own it is."""
+    m, n, k = 9, 64, 128
+    ops = linear_operands(m, n, k)
+    both = torch.randn(m, 2 * n, device="cuda").half()
+    bias = both[0, n:]
+    want = dg.linear(*ops, bias=bias.clone())
+    keep = both[:, n:].clone()
+    got = dg.linear(*ops, both[:, :n], bias=bias)
+    assert torch.equal(got, want) and torch.equal(both[:, n:], keep)
+    with pytest.raises(ValueError, match="must not overlap bias"):
+        dg.linear(*ops, both[:, :n], bias=both[3, :n])
+    assert torch.equal(got, want)
