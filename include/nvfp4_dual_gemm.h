@@ -369,8 +369,8 @@ NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, int residual,
  * the i-th of gate_rows equal runs of rows (1: one gate for all; rows: one
  * for each).  The stream x, y, R, Z have one type (F32, F16 or BF16) and
  * their own row pitches in elements (multiples of 8 and >= D; F32: of 4).  R
- * and Z may each be x or y, but must not overlap one another or the gate, nor
- * x or y in part.  Weights and biases are F32 or of the stream's type
+ * and Z may each be x or y, but must not overlap one another, the gate or a
+ * weight, nor x or y in part; codes and sf overlap nothing.  Weights and biases are F32 or of the stream's type
  * (w_dtype).  Outputs of z, either or none:
  *   Z              in the stream's type;
  *   codes and sf   NVFP4 for the next product: [rows, D/2] e2m1 codes and

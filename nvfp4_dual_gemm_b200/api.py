@@ -362,8 +362,8 @@ def block_norm(x, y=None, *, weight=None, bias=None, post_weight=None,
     type for all).  ``gate`` [G, D] (or [D]) holds one gate for each of G
     equal runs of rows: 1 for a channel gate, the batch for one a sample, the
     rows for one a row.  ``R`` and ``Z`` are allocated when not given; each
-    may be x or y itself, but not overlap them in part, nor the other or the
-    gate.  [rows, D] tensors may have strided rows (16-byte pitches).
+    may be x or y itself, but not overlap them in part, nor the other, the
+    gate or a weight.  [rows, D] tensors may have strided rows (16-byte pitches).
     D % 8 == 0 up to 32768.  Inference only (``nvfp4_block_norm_run``)."""
     return _lib.ext().block_norm(x, y, weight, bias, post_weight, post_bias,
                                  gate, scale, kind, eps, post, pre, R, Z,

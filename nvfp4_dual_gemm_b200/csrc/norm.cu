@@ -823,16 +823,42 @@ int check_norm(const nvfp4_block_norm_args* a) {
     return host_fail(NVFP4DG_ERR_INVALID,
                      "R and Z must each be x or y themselves or overlap "
                      "neither");
-  if (a->gate != nullptr) {
-    const uintptr_t g0 = reinterpret_cast<uintptr_t>(a->gate);
-    const uintptr_t g1 = g0 + static_cast<size_t>(a->gate_rows) * a->D * e;
-    auto meets = [&](const void* p, long long ld) {
-      const uintptr_t q = reinterpret_cast<uintptr_t>(p);
-      return p != nullptr &&
-             q < g1 && g0 < q + ((a->rows - 1) * ld + a->D) * e;
-    };
-    if (meets(r, a->ldr) || meets(a->Z, a->ldz))
-      return host_fail(NVFP4DG_ERR_INVALID, "gate must not overlap R or Z");
+  // what other rows' CTAs read, and what only they write
+  const long long w = (a->w_dtype == NVFP4DG_DTYPE_F32 ? 4ll : 2ll) * a->D;
+  struct Bytes {
+    const char* name;
+    const void* p;
+    long long n;
+  };
+  const Bytes shared[] = {
+      {"weight", a->weight, w},
+      {"bias", a->bias, w},
+      {"post_weight", a->post_weight, w},
+      {"post_bias", a->post_bias, w},
+      {"gate", a->gate, a->gate != nullptr ? a->gate_rows * (a->D * e) : 0},
+  };
+  for (const Bytes& in : shared)
+    if (host_meets(in.p, in.n, r, a->ldr * e, a->rows, a->D * e) ||
+        host_meets(in.p, in.n, a->Z, a->ldz * e, a->rows, a->D * e))
+      return host_fail(NVFP4DG_ERR_INVALID,
+                       std::string(in.name) + " must not overlap R or Z");
+  if (a->codes != nullptr) {
+    const Bytes outs[] = {
+        {"codes", a->codes, a->rows * (a->D / 2ll)},
+        {"sf", a->sf, (a->rows + 127ll) / 128 * (a->D / 64) * kAtomBytes}};
+    bool meets = host_meets(outs[0].p, outs[0].n, outs[1].p, outs[1].n, 1,
+                            outs[1].n);
+    for (const Bytes& out : outs) {
+      for (const Bytes& in : shared)
+        meets |= host_meets(out.p, out.n, in.p, in.n, 1, in.n);
+      for (int i = 0; i < 4; ++i)
+        meets |= host_meets(out.p, out.n, i == 2 ? r : mats[i], lds[i] * e,
+                            a->rows, a->D * e);
+    }
+    if (meets)
+      return host_fail(NVFP4DG_ERR_INVALID,
+                       "codes and sf must not overlap one another or any "
+                       "other tensor");
   }
   return NVFP4DG_OK;
 }

@@ -261,3 +261,33 @@ def test_linear_grouped_refuses_a_c_that_meets_a_later_groups_weights():
         a = {**kw, name: c + 16 - 2 * size}
         assert run_grouped([1, 1], **a) == _lib.ERR_INVALID
         assert "C must not overlap " + name in _lib.last_error()
+
+
+@pytest.mark.parametrize("out", ["R", "Z"])
+@pytest.mark.parametrize("where", [0, 128, 384, -16])
+@pytest.mark.parametrize("name", ["weight", "bias", "post_weight",
+                                  "post_bias"])
+def test_block_norm_refuses_outputs_over_its_weights(name, where, out):
+    kw = dict(x=FAR, y=2 * FAR, R=3 * FAR, Z=4 * FAR, post=1)
+    kw[name] = kw[out] + where
+    a = norm_args(**kw)
+    assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+        _lib.ERR_INVALID
+    assert name + " must not overlap" in _lib.last_error()
+
+
+@pytest.mark.parametrize("out,size", [("codes", 4 * 32), ("sf", 512)])
+@pytest.mark.parametrize("name", ["x", "y", "R", "Z", "weight", "bias",
+                                  "post_weight", "post_bias", "gate"])
+def test_block_norm_refuses_codes_over_anything_else(name, out, size):
+    kw = dict(x=FAR, y=2 * FAR, R=3 * FAR, Z=4 * FAR, codes=5 * FAR,
+              sf=6 * FAR, weight=7 * FAR, bias=8 * FAR, post_weight=9 * FAR,
+              post_bias=10 * FAR, gate=11 * FAR, gate_rows=2, post=1)
+    for at in (kw[name], kw[name] - size + 16):
+        a = norm_args(**{**kw, out: at})
+        assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+            _lib.ERR_INVALID
+        assert "codes and sf must not overlap" in _lib.last_error()
+    a = norm_args(**{**kw, "sf": kw["codes"] + 112})
+    assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
+        _lib.ERR_INVALID

@@ -36,3 +36,22 @@ def test_c_beside_the_bias_in_one_buffer():
     with pytest.raises(ValueError, match="must not overlap bias"):
         dg.linear(*ops, both[:, :n], bias=both[3, :n])
     assert torch.equal(got, want)
+
+
+def test_norm_outputs_beside_gate_and_weight_in_one_buffer():
+    """Gate and weights in the columns that a strided R leaves out are no
+    overlap; in its own they are."""
+    rows, d = 7, 128
+    x, y = (torch.randn(rows, d, device="cuda").half() for _ in range(2))
+    both = torch.randn(rows, 2 * d, device="cuda").half()
+    gate, w = both[0, d:], both[5, d:]
+    want = dg.block_norm(x, y, gate=gate.clone(), weight=w.clone())
+    keep = both[:, d:].clone()
+    r, z = dg.block_norm(x, y, gate=gate, weight=w, R=both[:, :d])
+    assert torch.equal(r, want[0]) and torch.equal(z, want[1])
+    assert torch.equal(both[:, d:], keep)
+    for kw in (dict(gate=both[2, :d]), dict(weight=both[2, :d]),
+               dict(post_bias=both[6, :d])):
+        with pytest.raises(ValueError, match="must not overlap R or Z"):
+            dg.block_norm(x, y, R=both[:, :d], **kw)
+    assert torch.equal(r, want[0])
