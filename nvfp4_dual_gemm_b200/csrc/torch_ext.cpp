@@ -14,6 +14,7 @@
 // Invalid arguments raise ValueError; CUDA and device failures RuntimeError.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
@@ -231,11 +232,15 @@ at::Tensor dual_gemm(const at::Tensor& A, const at::Tensor& B1,
 using OptTensor = c10::optional<at::Tensor>;
 
 // These operators have no gradient: rather than cut one silently, they refuse
-// inputs that ask for it.
+// inputs that ask for it, by a backward pass or by a forward-mode tangent.
 void no_grad_input(const char* name, const at::Tensor& t) {
   if (t.requires_grad() && at::GradMode::is_enabled())
     bad(std::string(name) + " requires grad; this operator is inference only "
         "(use torch.no_grad())");
+  if (t._fw_grad(/*level=*/0).defined() &&
+      c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    bad(std::string(name) + " has a forward-mode tangent; this operator is "
+        "inference only (use torch.autograd.forward_ad.unpack_dual)");
 }
 
 void on_device(const char* name, const at::Tensor& t, const at::Device& dev) {

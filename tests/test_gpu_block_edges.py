@@ -55,3 +55,53 @@ def test_norm_outputs_beside_gate_and_weight_in_one_buffer():
         with pytest.raises(ValueError, match="must not overlap R or Z"):
             dg.block_norm(x, y, R=both[:, :d], **kw)
     assert torch.equal(r, want[0])
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    def refused():
+        return pytest.raises(ValueError, match="inference only")
+    n, half = 128, dict(dtype=torch.float16, device="cuda")
+    ops = linear_operands(4, n, 128)
+    f8 = ops[3].view(torch.float8_e4m3fn)
+    x, y, w = (torch.randn(4, n, **half), torch.randn(4, n, **half),
+               torch.ones(n, device="cuda"))
+    want, norm = dg.linear(*ops, residual=x), dg.block_norm(x, y, weight=w)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        for kw in (dict(bias=dual(w)), dict(residual=dual(x)),
+                   dict(row_scale=dual(torch.ones(4, device="cuda")))):
+            with torch.no_grad(), refused():
+                dg.linear(*ops, **kw)
+        with refused():
+            dg.linear(*ops, dual(x.clone()))
+        with refused():
+            dg.linear_grouped(*ops, x.clone(), [4], bias=dual(w[None]))
+        for args, kw in (((dual(x),), {}), ((x, dual(y)), {}),
+                         ((x,), dict(weight=dual(w))),
+                         ((x,), dict(bias=dual(w))),
+                         ((x, y), dict(post_weight=dual(w))),
+                         ((x, y), dict(gate=dual(x[0].clone()))),
+                         ((x, y), dict(R=dual(x.clone())))):
+            with refused():
+                dg.block_norm(*args, **kw)
+            with refused():
+                dg.block_norm_nvfp4(*args, **kw)
+        # with the tangent taken off, or with forward mode off as inside a
+        # custom function's forward
+        assert torch.equal(dg.linear(*ops[:3], f8,
+                                     residual=fw.unpack_dual(dual(x)).primal),
+                           want)
+
+        class Norm(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, v):
+                return dg.block_norm(v, y, weight=w)[1]
+
+            @staticmethod
+            def jvp(ctx, t):
+                return t
+        assert torch.equal(fw.unpack_dual(Norm.apply(dual(x))).primal,
+                           norm[1])
