@@ -55,6 +55,14 @@ def _stream(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _wrote(*tensors: torch.Tensor) -> None:
+    """Tensors of the caller's were written in place: autograd's check of the
+    tensors it saved goes by their version (inference tensors have none)."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _check_bytes(name: str, t: torch.Tensor, cuda: bool = True) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -188,6 +196,7 @@ def dual_gemm_nvfp4(A, B1, B2, SFA, SFB1, SFB2, Cq=None, SFC=None, *,
     holds L blocked layouts one after another."""
     M, N, K, L = _check_inputs(A, B1, B2, SFA, SFB1, SFB2, cuda=True)
     dev = A.device
+    given = [t for t in (Cq, SFC) if t is not None]
     if Cq is None:
         Cq = (torch.empty((M, N // 2), dtype=torch.uint8, device=dev)
               if L == 1 else
@@ -209,6 +218,7 @@ def dual_gemm_nvfp4(A, B1, B2, SFA, SFB1, SFB2, Cq=None, SFC=None, *,
             _ptr(A), _ptr(B1), _ptr(B2), _ptr(SFA), _ptr(SFB1), _ptr(SFB2),
             _ptr(Cq), _ptr(SFC), M, N, K, L, flags, _stream(dev))
     _lib.check(rc, "nvfp4_dual_gemm_run_nvfp4_out")
+    _wrote(*given)
     return Cq, SFC
 
 
@@ -282,6 +292,7 @@ def dual_gemm_grouped(A, B1, B2, SFA, SFB1, SFB2, C, group_rows,
             None if workspace is None else _ptr(workspace),
             0 if workspace is None else workspace.numel(), _stream(dev))
     _lib.check(rc, "nvfp4_dual_gemm_run_grouped")
+    _wrote(C)
     return C
 
 
@@ -439,6 +450,7 @@ def dual_gemm_host(A, B1, B2, SFA, SFB1, SFB2, C, *, flags: int = 0,
             _ptr(C), M, N, K, 1, flags, slabs, _ptr(buf),
             buf.numel() * buf.element_size(), stream)
     _lib.check(rc, "nvfp4_dual_gemm_run_host")
+    _wrote(C)
     return C
 
 

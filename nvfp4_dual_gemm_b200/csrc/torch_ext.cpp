@@ -158,6 +158,12 @@ void check_status(int rc, const char* what) {
   throw std::runtime_error(msg);
 }
 
+// A caller's tensor was written in place: autograd's check of the tensors it
+// saved goes by their version.  (Inference tensors have none.)
+void wrote(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor run(const at::Tensor& A, const at::Tensor& B1, const at::Tensor& B2,
                const at::Tensor& SFA, const at::Tensor& SFB1,
                const at::Tensor& SFB2, const at::Tensor& C, int64_t flags,
@@ -184,6 +190,7 @@ at::Tensor run(const at::Tensor& A, const at::Tensor& B1, const at::Tensor& B2,
         static_cast<size_t>(ws->numel()) * ws->element_size(), stream);
   }
   check_status(rc, "nvfp4_dual_gemm_run");
+  wrote(C);
   return C;
 }
 
@@ -413,6 +420,7 @@ at::Tensor linear(const at::Tensor& A, const at::Tensor& B,
       nvfp4_linear_run(
           &a, at::cuda::getCurrentCUDAStream(A.device().index()).stream()),
       "nvfp4_linear_run");
+  if (C_in.has_value()) wrote(C);
   return C;
 }
 
@@ -502,6 +510,7 @@ at::Tensor linear_grouped(const at::Tensor& A, const at::Tensor& B,
           dim32("groups", G), on_dev ? 1 : 0,
           at::cuda::getCurrentCUDAStream(A.device().index()).stream()),
       "nvfp4_linear_run_grouped");
+  wrote(C);
   return C;
 }
 
@@ -650,6 +659,8 @@ NormOut norm(const at::Tensor& x_in, const OptTensor& y_in,
   check_status(nvfp4_block_norm_run(
                    &a, at::cuda::getCurrentCUDAStream(dev.index()).stream()),
                "nvfp4_block_norm_run");
+  if (R_in.has_value()) wrote(out.R);
+  if (Z_in.has_value()) wrote(out.Z);
   return out;
 }
 

@@ -105,3 +105,58 @@ def test_forward_mode_tangents_are_refused():
                 return t
         assert torch.equal(fw.unpack_dual(Norm.apply(dual(x))).primal,
                            norm[1])
+
+
+def test_outputs_of_the_callers_raise_their_version():
+    n, half = 256, dict(dtype=torch.float16, device="cuda")
+    ops = linear_operands(4, n, n)
+    x, y = torch.randn(4, n, **half), torch.randn(4, n, **half)
+    d = dg.generate_input(4, n, 2 * n)
+    a, b1, b2, sfa, sfb1, sfb2 = (d[i] for i in (0, 1, 2, 6, 7, 8))
+    c = d[9].squeeze(2)
+    cq, sfc = dg.dual_gemm_nvfp4(a, b1, b2, sfa, sfb1, sfb2)
+    host = [t.cpu().pin_memory() for t in (*(t.view(torch.uint8) for t in (
+        a, b1, b2, sfa, sfb1, sfb2)), d[9])]
+    calls = {
+        "linear": (lambda t: dg.linear(*ops, t), x.clone()),
+        "in place": (lambda t: dg.linear(*ops, t, residual=t), x.clone()),
+        "linear_grouped": (lambda t: dg.linear_grouped(*ops, t, [4]),
+                           x.clone()),
+        "R": (lambda t: dg.block_norm(x, y, R=t), x.clone()),
+        "Z": (lambda t: dg.block_norm(x, y, Z=t), x.clone()),
+        "R of nvfp4": (lambda t: dg.block_norm_nvfp4(t, y, R=t), x.clone()),
+        "dual_gemm": (lambda t: dg.dual_gemm(a, b1, b2, sfa, sfb1, sfb2, t),
+                      c.clone()),
+        "custom_kernel": (lambda t: dg.custom_kernel((*d[:9], t)), c.clone()),
+        "dual_gemm_grouped": (lambda t: dg.dual_gemm_grouped(
+            a, b1, b2, sfa, sfb1, sfb2, t, [4]), c.clone()),
+        "Cq": (lambda t: dg.dual_gemm_nvfp4(a, b1, b2, sfa, sfb1, sfb2, t),
+               cq),
+        "SFC": (lambda t: dg.dual_gemm_nvfp4(a, b1, b2, sfa, sfb1, sfb2,
+                                             SFC=t), sfc),
+        "dual_gemm_host": (lambda t: dg.dual_gemm_host(*host[:6], t),
+                           host[6]),
+    }
+    for name, (call, t) in calls.items():
+        before, reads = t._version, (x._version, y._version)
+        call(t)
+        assert t._version > before, name
+        assert (x._version, y._version) == reads, name
+        view = t[:2]
+        call(t)
+        assert view._version == t._version, name
+    with torch.inference_mode():
+        t = x.clone()
+        dg.linear(*ops, t, residual=t)
+        dg.block_norm(t, y, R=t)
+    dg.linear(*ops, t)  # and outside of it: an inference tensor has no version
+    torch.cuda.synchronize()
+
+
+def test_a_saved_tensor_that_is_overwritten_fails_its_backward():
+    w = torch.randn(4, 64, device="cuda", requires_grad=True)
+    s = torch.exp(w)  # backward reads s
+    dg.block_norm(s.detach(), torch.ones(4, 64, device="cuda"),
+                  R=s.detach())
+    with pytest.raises(RuntimeError, match="inplace"):
+        s.sum().backward()
