@@ -63,6 +63,13 @@ def _wrote(*tensors: torch.Tensor) -> None:
             torch.autograd.graph.increment_version(t)
 
 
+def _flag_bits(flags: int) -> int:
+    """``flags`` for ctypes, which would cut it to 32 bits."""
+    if not 0 <= flags < 1 << 32:
+        raise ValueError(f"flags must be 32 bits, got {flags}")
+    return flags
+
+
 def _check_bytes(name: str, t: torch.Tensor, cuda: bool = True) -> None:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -216,7 +223,8 @@ def dual_gemm_nvfp4(A, B1, B2, SFA, SFB1, SFB2, Cq=None, SFC=None, *,
     with torch.cuda.device(dev):
         rc = lib.nvfp4_dual_gemm_run_nvfp4_out(
             _ptr(A), _ptr(B1), _ptr(B2), _ptr(SFA), _ptr(SFB1), _ptr(SFB2),
-            _ptr(Cq), _ptr(SFC), M, N, K, L, flags, _stream(dev))
+            _ptr(Cq), _ptr(SFC), M, N, K, L, _flag_bits(flags),
+            _stream(dev))
     _lib.check(rc, "nvfp4_dual_gemm_run_nvfp4_out")
     _wrote(*given)
     return Cq, SFC
@@ -238,7 +246,8 @@ def grouped_workspace_size(group_rows, N: int, K: int,
     rows = [int(n) for n in group_rows]
     lib = _lib.load()
     return int(lib.nvfp4_dual_gemm_grouped_workspace_size(
-        (ctypes.c_int * len(rows))(*rows), len(rows), N, K, flags))
+        (ctypes.c_int * len(rows))(*rows), len(rows), N, K,
+        _flag_bits(flags)))
 
 
 def dual_gemm_grouped(A, B1, B2, SFA, SFB1, SFB2, C, group_rows,
@@ -288,7 +297,7 @@ def dual_gemm_grouped(A, B1, B2, SFA, SFB1, SFB2, C, group_rows,
     with torch.cuda.device(dev):
         rc = lib.nvfp4_dual_gemm_run_grouped(
             _ptr(A), _ptr(B1), _ptr(B2), _ptr(SFA), _ptr(SFB1), _ptr(SFB2),
-            _ptr(C), arr(*rows), arr(*row0), G, N, K, flags,
+            _ptr(C), arr(*rows), arr(*row0), G, N, K, _flag_bits(flags),
             None if workspace is None else _ptr(workspace),
             0 if workspace is None else workspace.numel(), _stream(dev))
     _lib.check(rc, "nvfp4_dual_gemm_run_grouped")
@@ -346,11 +355,13 @@ def linear_plan(M: int, N: int, K: int, residual: bool = False,
     """The schedule :func:`linear` would use, with a residual or without:
     tokens per tile (256: 2-SM pairs), CTAs that share a tile's K range
     (``split``) and CTAs in all (host-only; needs no GPU)."""
+    if max(M, N, K, num_sms) > 1 << 30:
+        raise ValueError("M, N and K must not exceed 2^30")
     lib = _lib.load()
     tokens, split, grid = (ctypes.c_int() for _ in range(3))
-    rc = lib.nvfp4_linear_plan(M, N, K, int(residual), flags, num_sms,
-                               ctypes.byref(tokens), ctypes.byref(split),
-                               ctypes.byref(grid))
+    rc = lib.nvfp4_linear_plan(M, N, K, int(residual), _flag_bits(flags),
+                               num_sms, ctypes.byref(tokens),
+                               ctypes.byref(split), ctypes.byref(grid))
     _lib.check(rc, "nvfp4_linear_plan")
     return {"tokens": tokens.value, "split": split.value, "grid": grid.value}
 
@@ -447,7 +458,7 @@ def dual_gemm_host(A, B1, B2, SFA, SFB1, SFB2, C, *, flags: int = 0,
             buf = staging
         rc = lib.nvfp4_dual_gemm_run_host(
             _ptr(A), _ptr(B1), _ptr(B2), _ptr(SFA), _ptr(SFB1), _ptr(SFB2),
-            _ptr(C), M, N, K, 1, flags, slabs, _ptr(buf),
+            _ptr(C), M, N, K, 1, _flag_bits(flags), slabs, _ptr(buf),
             buf.numel() * buf.element_size(), stream)
     _lib.check(rc, "nvfp4_dual_gemm_run_host")
     _wrote(C)
@@ -477,7 +488,8 @@ def workspace_size(M: int, N: int, K: int, flags: int = 0,
     dev = torch.device("cuda", torch.cuda.current_device()
                        if device is None else torch.device(device).index or 0)
     with torch.cuda.device(dev):
-        n = lib.nvfp4_dual_gemm_workspace_size(M, N, K, L, flags)
+        n = lib.nvfp4_dual_gemm_workspace_size(M, N, K, L,
+                                               _flag_bits(flags))
     msg = _lib.last_error()
     if n == 0 and msg:
         raise RuntimeError(msg)
@@ -488,10 +500,10 @@ def plan(M: int, N: int, K: int, flags: int = 0, num_sms: int = 148) -> dict:
     """The schedule the library would use (host-only; needs no GPU)."""
     lib = _lib.load()
     bn, ctas, grid, dp, sk, split = (ctypes.c_int() for _ in range(6))
-    rc = lib.nvfp4_dual_gemm_plan(M, N, K, flags, num_sms, ctypes.byref(bn),
-                                  ctypes.byref(ctas), ctypes.byref(grid),
-                                  ctypes.byref(dp), ctypes.byref(sk),
-                                  ctypes.byref(split))
+    rc = lib.nvfp4_dual_gemm_plan(M, N, K, _flag_bits(flags), num_sms,
+                                  ctypes.byref(bn), ctypes.byref(ctas),
+                                  ctypes.byref(grid), ctypes.byref(dp),
+                                  ctypes.byref(sk), ctypes.byref(split))
     _lib.check(rc, "nvfp4_dual_gemm_plan")
     return {"bn": bn.value, "ctas": ctas.value, "grid": grid.value,
             "dp_tiles": dp.value, "sk_tiles": sk.value,
@@ -503,7 +515,8 @@ def plan_work(M: int, N: int, K: int, cta: int, flags: int = 0,
     """Work records (tile, kb_begin, kb_end, slot) of one work unit (a CTA or
     a 2-SM CTA pair; host-only)."""
     lib = _lib.load()
-    n = lib.nvfp4_dual_gemm_plan_work(M, N, K, flags, num_sms, cta, None, 0)
+    n = lib.nvfp4_dual_gemm_plan_work(M, N, K, _flag_bits(flags), num_sms,
+                                      cta, None, 0)
     if n < 0:
         raise ValueError(_lib.last_error())
     buf = (ctypes.c_int * (4 * max(n, 1)))()

@@ -41,6 +41,12 @@ std::string dims(const at::Tensor& t) {
   return s + (t.dim() == 1 ? ",)" : ")");
 }
 
+unsigned flag_bits(int64_t flags) {
+  if (flags < 0 || flags > int64_t{UINT32_MAX})
+    bad("flags must be 32 bits, got " + std::to_string(flags));
+  return static_cast<unsigned>(flags);
+}
+
 void check_bytes(const char* name, const at::Tensor& t) {
   if (t.element_size() != 1)
     bad(std::string(name) +
@@ -178,7 +184,7 @@ at::Tensor run(const at::Tensor& A, const at::Tensor& B1, const at::Tensor& B2,
                              C.data_ptr(), static_cast<int>(p.M),
                              static_cast<int>(p.N), static_cast<int>(p.K),
                              static_cast<int>(p.L),
-                             static_cast<unsigned>(flags), stream);
+                             flag_bits(flags), stream);
   } else {
     if (ws->device() != C.device() || !ws->is_contiguous())
       bad("workspace must be a contiguous tensor on C's device");
@@ -186,7 +192,7 @@ at::Tensor run(const at::Tensor& A, const at::Tensor& B1, const at::Tensor& B2,
         A.data_ptr(), B1.data_ptr(), B2.data_ptr(), SFA.data_ptr(),
         SFB1.data_ptr(), SFB2.data_ptr(), C.data_ptr(), static_cast<int>(p.M),
         static_cast<int>(p.N), static_cast<int>(p.K), static_cast<int>(p.L),
-        static_cast<unsigned>(flags), ws->data_ptr(),
+        flag_bits(flags), ws->data_ptr(),
         static_cast<size_t>(ws->numel()) * ws->element_size(), stream);
   }
   check_status(rc, "nvfp4_dual_gemm_run");
@@ -373,7 +379,7 @@ nvfp4_linear_args linear_args(const at::Tensor& A, const at::Tensor& B,
   }
   a.activation = activation_code(activation);
   a.alpha = static_cast<float>(alpha);
-  a.flags = static_cast<unsigned>(flags);
+  a.flags = flag_bits(flags);
   return a;
 }
 
@@ -609,7 +615,7 @@ NormOut norm(const at::Tensor& x_in, const OptTensor& y_in,
   if (!(eps >= 0)) bad("eps must not be negative");
   a.eps = static_cast<float>(eps);
   a.scale = static_cast<float>(scale);
-  a.flags = static_cast<unsigned>(flags);
+  a.flags = flag_bits(flags);
   at::Tensor y, g, r, z;
   if (y_in.has_value()) {
     y = same("y", *y_in);

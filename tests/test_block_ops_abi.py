@@ -291,3 +291,22 @@ def test_block_norm_refuses_codes_over_anything_else(name, out, size):
     a = norm_args(**{**kw, "sf": kw["codes"] + 112})
     assert _lib.load().nvfp4_block_norm_run(ctypes.byref(a), None) == \
         _lib.ERR_INVALID
+
+
+@pytest.mark.parametrize("flags", [1 << 32, (1 << 32) + 1, -1, -(1 << 32)])
+def test_flags_beyond_32_bits_are_refused(flags):
+    for call in (lambda: dg.linear_plan(4, 128, 256, flags=flags),
+                 lambda: dg.plan(128, 256, 512, flags),
+                 lambda: dg.plan_work(128, 256, 512, 0, flags),
+                 lambda: dg.grouped_workspace_size([4], 128, 256, flags)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
+
+
+def test_plan_refuses_sizes_beyond_32_bits():
+    for size in ((4 + (1 << 32), 128, 256), (4, 128 + (1 << 32), 256),
+                 (4, 128, 256 + (1 << 32))):
+        with pytest.raises(ValueError):
+            dg.linear_plan(*size)
+    with pytest.raises(ValueError):
+        dg.linear_plan(4, 128, 256, num_sms=148 + (1 << 32))

@@ -160,3 +160,17 @@ def test_a_saved_tensor_that_is_overwritten_fails_its_backward():
                   R=s.detach())
     with pytest.raises(RuntimeError, match="inplace"):
         s.sum().backward()
+
+
+@pytest.mark.parametrize("flags", [1 << 32, (1 << 32) + 4, -1])
+def test_flags_beyond_32_bits_are_refused(flags):
+    ops = linear_operands(4, 256, 256)
+    x = torch.randn(4, 256, device="cuda").half()
+    for call in (lambda: dg.linear(*ops, flags=flags),
+                 lambda: dg.linear_grouped(*ops, x, [4], flags=flags),
+                 lambda: dg.block_norm(x, flags=flags),
+                 lambda: dg.block_norm_nvfp4(x, flags=flags),
+                 lambda: dg.dual_gemm(ops[0], ops[1], ops[1], ops[2], ops[3],
+                                      ops[3], x, flags=flags)):
+        with pytest.raises(ValueError, match="32 bits"):
+            call()
