@@ -303,6 +303,11 @@ NVFP4DG_API int nvfp4_scales_from_blocked(const void* blocked, int rows, int K,
 #define NVFP4DG_LINEAR_PAIR (1u << 3) /* 256 x 256 tiles of two SMs */
 #define NVFP4DG_LINEAR_SPLIT_MASK 0x700u
 #define NVFP4DG_LINEAR_SPLIT(log2) ((1u + (log2)) << 8)
+#define NVFP4DG_LINEAR_TEST_NO_PAIR (1u << 25) /* test hook, never for
+                                          production: as if this build's pair
+                                          kernel could not be launched, which
+                                          leaves its problems to the other
+                                          tiles */
 
 typedef struct {
   const void* A;

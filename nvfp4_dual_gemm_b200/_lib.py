@@ -50,6 +50,7 @@ LINEAR_TOKENS32 = 1 << 0
 LINEAR_TOKENS64 = 1 << 1
 LINEAR_TOKENS128 = 1 << 2
 LINEAR_PAIR = 1 << 3
+LINEAR_TEST_NO_PAIR = 1 << 25
 
 
 def linear_split(ctas: int) -> int:

@@ -1707,10 +1707,10 @@ double linear_cost(int tn, double kb, double waves, bool split, int tokens,
 }
 
 // `mts`: token tiles of 32, 64, 128 and 256 tokens (of all groups); `tokens`:
-// of all of them.
+// of all of them; `pairs`: whether pair tiles may be taken.
 LinearPlan plan_linear(const long long (&mts)[4], long long tokens, int N,
                        int K, int groups, bool residual, unsigned flags,
-                       int sms) {
+                       int sms, bool pairs) {
   const unsigned forced_tile =
       flags & (NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
                NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR);
@@ -1723,7 +1723,7 @@ LinearPlan plan_linear(const long long (&mts)[4], long long tokens, int N,
     if (forced_tile && !(forced_tile & (1u << i))) continue;
     const int tn = 32 << i;
     const int ctas = tn == 256 ? 2 : 1;
-    if (sms < ctas) continue;
+    if (tn == 256 && (sms < 2 || !pairs)) continue;
     LinearPlan pl{};
     pl.tn = tn;
     pl.kblocks = tn <= 64 ? (K + 511) / 512 : kb256;
@@ -1810,28 +1810,36 @@ int launch_linear(const LinearParams& kp, const LinearPlan& pl,
   return NVFP4DG_OK;
 }
 
+// Whether linear_pair_kernel can be launched: its warpgroups' shares of the
+// registers come out of what the launch allocates, and only a build with
+// exactly that many lets every increase end.
 template <typename T>
-int launch_pair(const LinearParams& kp, const LinearPlan& pl,
-                const CUtensorMap& tw, const CUtensorMap& tx,
-                const CUtensorMap& tc, int dev, unsigned flags,
-                cudaStream_t stream) {
-  static std::atomic<unsigned long long> ready{0};
+int pair_usable(int dev, bool* usable) {
+  static std::atomic<unsigned long long> checked{0}, fits{0};
   auto kernel = linear_pair_kernel<T>;
   const unsigned long long bit = 1ull << (dev & 63);
-  if (!(ready.load() & bit)) {
+  if (!(checked.load() & bit)) {
     cudaFuncAttributes fa;
     cudaError_t e = cudaFuncGetAttributes(&fa, kernel);
     if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncGetAttributes");
-    // the warpgroups' shares come out of what the launch allocates
-    if (fa.numRegs != kPairRegs)
-      return host_fail(NVFP4DG_ERR_CUDA,
-                       "linear_pair_kernel was built with " +
-                           std::to_string(fa.numRegs) + " registers");
-    e = cudaFuncSetAttribute(
-        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
-    if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
-    ready.fetch_or(bit);
+    if (fa.numRegs == kPairRegs) {
+      e = cudaFuncSetAttribute(
+          kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+      if (e != cudaSuccess) return host_cuda_fail(e, "cudaFuncSetAttribute");
+      fits.fetch_or(bit);
+    }
+    checked.fetch_or(bit);
   }
+  *usable = (fits.load() & bit) != 0;
+  return NVFP4DG_OK;
+}
+
+// (pair_usable has been asked)
+template <typename T>
+int launch_pair(const LinearParams& kp, const LinearPlan& pl,
+                const CUtensorMap& tw, const CUtensorMap& tx,
+                const CUtensorMap& tc, unsigned flags, cudaStream_t stream) {
+  auto kernel = linear_pair_kernel<T>;
   LinearParams p = kp;
   p.m_tiles = (p.M + 255) / 256;
   p.n_tiles = (p.N + 255) / 256;
@@ -1863,6 +1871,7 @@ int check_linear_flags(unsigned flags) {
   const unsigned known = NVFP4DG_LINEAR_TOKENS32 | NVFP4DG_LINEAR_TOKENS64 |
                          NVFP4DG_LINEAR_TOKENS128 | NVFP4DG_LINEAR_PAIR |
                          NVFP4DG_LINEAR_SPLIT_MASK |
+                         NVFP4DG_LINEAR_TEST_NO_PAIR |
                          NVFP4DG_FLAG_SYNC_CHECK | NVFP4DG_FLAG_NO_PDL;
   if (flags & ~known)
     return host_fail(NVFP4DG_ERR_INVALID, "unknown flag bits");
@@ -2013,10 +2022,24 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
   if ((rc = check_linear_overlap(a, groups))) return rc;
   HostDevice dev;
   if ((rc = host_device(&dev))) return rc;
-  LinearPlan pl = plan_linear(mt, tokens, a->N, a->K, groups,
-                              a->residual != nullptr, a->flags, dev.sms);
+  const bool bf = a->c_dtype == NVFP4DG_DTYPE_BF16;
+  auto plan = [&](bool pairs) {
+    return plan_linear(mt, tokens, a->N, a->K, groups, a->residual != nullptr,
+                       a->flags, dev.sms, pairs);
+  };
+  LinearPlan pl = plan(true);
   if (pl.tn == 0)
     return host_fail(NVFP4DG_ERR_INVALID, "pairs need two SMs");
+  if (pl.tn == 256) {
+    bool usable = false;
+    if ((rc = bf ? pair_usable<__nv_bfloat16>(dev.id, &usable)
+                 : pair_usable<__half>(dev.id, &usable)))
+      return rc;
+    if (!usable || (a->flags & NVFP4DG_LINEAR_TEST_NO_PAIR)) pl = plan(false);
+    if (pl.tn == 0)
+      return host_fail(NVFP4DG_ERR_UNSUPPORTED,
+                       "this build's pair kernel cannot be launched");
+  }
   // tiles counted by the kernel: a full grid
   if (groups > 0 && on_device)
     pl.grid = pl.tn == 256 ? dev.sms / 2 * 2 : dev.sms;
@@ -2051,16 +2074,13 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
                           a->M * kb, &tx)))
     return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const bool bf = a->c_dtype == NVFP4DG_DTYPE_BF16;
   if (pl.tn == 256) {
     CUtensorMap tc;
     if ((rc = host_byte_map(a->C, a->M, 2ll * a->N, 2 * a->ldc, 128, 0, 0,
                             &tc)))
       return rc;
-    rc = bf ? launch_pair<__nv_bfloat16>(p, pl, tw, tx, tc, dev.id, a->flags,
-                                         stream)
-            : launch_pair<__half>(p, pl, tw, tx, tc, dev.id, a->flags,
-                                  stream);
+    rc = bf ? launch_pair<__nv_bfloat16>(p, pl, tw, tx, tc, a->flags, stream)
+            : launch_pair<__half>(p, pl, tw, tx, tc, a->flags, stream);
   } else if (pl.tn == 32)
     rc = bf ? launch_linear<__nv_bfloat16, 32>(p, pl, tw, tx, dev.id,
                                                a->flags, stream)
@@ -2124,7 +2144,8 @@ int nvfp4_linear_plan(int M, int N, int K, int residual, unsigned flags,
     const long long mts[4] = {(M + 31ll) / 32, (M + 63ll) / 64,
                               (M + 127ll) / 128, (M + 255ll) / 256};
     const nvfp4dg::LinearPlan pl = nvfp4dg::plan_linear(
-        mts, M, N, K, 0, residual != 0, flags, num_sms);
+        mts, M, N, K, 0, residual != 0, flags, num_sms,
+        !(flags & NVFP4DG_LINEAR_TEST_NO_PAIR));
     if (pl.tn == 0)
       return nvfp4dg::host_fail(NVFP4DG_ERR_INVALID, "pairs need two SMs");
     if (tokens_out) *tokens_out = pl.tn;

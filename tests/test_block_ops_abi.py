@@ -310,3 +310,10 @@ def test_plan_refuses_sizes_beyond_32_bits():
             dg.linear_plan(*size)
     with pytest.raises(ValueError):
         dg.linear_plan(4, 128, 256, num_sms=148 + (1 << 32))
+
+
+def test_plan_without_pairs_takes_other_tiles():
+    for m, n, k in ((4096, 4096, 14336), (500, 8192, 7168), (2048, 2056, 2048)):
+        assert dg.linear_plan(m, n, k)["tokens"] == 256
+        pl = dg.linear_plan(m, n, k, flags=_lib.LINEAR_TEST_NO_PAIR)
+        assert pl["tokens"] in (32, 64, 128) and 1 <= pl["grid"] <= 148

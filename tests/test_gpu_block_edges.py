@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import nvfp4_dual_gemm_b200 as dg
+from nvfp4_dual_gemm_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +175,23 @@ def test_flags_beyond_32_bits_are_refused(flags):
                                       ops[3], x, flags=flags)):
         with pytest.raises(ValueError, match="32 bits"):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_without_its_pair_kernel_the_other_tiles_compute(dtype):
+    """A build whose pair kernel cannot be launched leaves its problems to the
+    128-token tiles, which round the same sums the same way."""
+    m, n, k = 2048, 2056, 2048
+    ops = linear_operands(m, n, k)
+    assert dg.linear_plan(m, n, k)["tokens"] == 256
+    flags = _lib.LINEAR_TEST_NO_PAIR | _lib.FLAG_SYNC_CHECK
+    want = dg.linear(*ops, dtype=dtype, flags=_lib.LINEAR_TOKENS128)
+    got = dg.linear(*ops, dtype=dtype, flags=flags)
+    assert torch.equal(got, want)
+    b, sfb = ops[1][None].permute(1, 2, 0), ops[3]
+    for counts in ([m], torch.tensor([m], dtype=torch.int32, device="cuda")):
+        got.zero_()
+        dg.linear_grouped(ops[0], b, ops[2], sfb, got, counts, flags=flags)
+        assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="pair kernel"):
+        dg.linear(*ops, dtype=dtype, flags=flags | _lib.LINEAR_PAIR)
