@@ -1,11 +1,16 @@
 """GPU tests of what the block operators' documentation allows at its edges:
 outputs beside their inputs in one buffer, tensors that autograd knows,
 schedules where a CTA's tiles belong to several groups, and many wide rows."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import nvfp4_dual_gemm_b200 as dg
 from nvfp4_dual_gemm_b200 import _lib
+from tests.test_gpu_block_norm import check, problem, reference
+from tests.test_gpu_linear import TILES, Groups
 
 pytestmark = pytest.mark.gpu
 
@@ -195,3 +200,125 @@ def test_without_its_pair_kernel_the_other_tiles_compute(dtype):
         assert torch.equal(got, want)
     with pytest.raises(RuntimeError, match="pair kernel"):
         dg.linear(*ops, dtype=dtype, flags=flags | _lib.LINEAR_PAIR)
+
+
+# boxed and row-by-row stores, groups that end within a tile and empty ones
+# alternate among the tiles of one CTA
+MIXED = [0, 300, 37, 128, 513, 0, 255, 129]
+
+
+@pytest.mark.parametrize("where", ["host", "device"])
+@pytest.mark.parametrize("tile", ["auto", "t32", "t64", "t128", "pair"])
+def test_grouped_tiles_of_several_groups_in_one_cta(tile, where):
+    """More tiles than workers: 162 of pairs, 490 of 128 tokens and more of
+    the others."""
+    p = Groups(MIXED, 4360, 576, seed=21)
+    rows = MIXED if where == "host" else torch.tensor(
+        MIXED, dtype=torch.int32, device="cuda")
+    p.run(rows, flags=TILES[tile])
+    p.check()
+
+
+def test_grouped_pairs_replayed_with_other_counts():
+    p = Groups(MIXED, 2312, 320, seed=22, cap=2304)
+    counts = torch.tensor(MIXED, dtype=torch.int32, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dg.linear_grouped(p.A, p.B, p.SFA, p.SFB, p.C, counts, bias=p.bias,
+                          activation="silu", row_scale=p.w,
+                          flags=_lib.LINEAR_PAIR)
+    for new in (MIXED, MIXED[::-1], [257, 1, 0, 511, 128, 64, 256, 5],
+                [0] * 7 + [1500], MIXED):
+        counts.copy_(torch.tensor(new, dtype=torch.int32))
+        p.C.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        p.check(new, dg.group_offsets(new))
+
+
+def test_grouped_pairs_on_two_streams():
+    p = Groups(MIXED, 2312, 320, seed=23)
+    args = (p.A, p.B, p.SFA, p.SFB)
+    kw = dict(bias=p.bias, activation="silu", row_scale=p.w,
+              flags=_lib.LINEAR_PAIR)
+    counts = torch.tensor(MIXED, dtype=torch.int32, device="cuda")
+    p.C.zero_()
+    dg.linear_grouped(*args, p.C, counts, **kw)
+    outs = [torch.zeros_like(p.C) for _ in range(16)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i, c in enumerate(outs):
+        with torch.cuda.stream(streams[i % 2]):
+            dg.linear_grouped(*args, c, counts, **kw)
+    torch.cuda.synchronize()
+    assert all(torch.equal(c, p.C) for c in outs)
+
+
+FIRST_PAIR_IN_CAPTURE = """
+import torch
+import nvfp4_dual_gemm_b200 as dg
+from nvfp4_dual_gemm_b200 import _lib
+u8 = dict(dtype=torch.uint8, device="cuda")
+a = torch.randint(0, 256, (300, 128), **u8)
+b = torch.randint(0, 256, (520, 128), **u8)
+sfa, sfb = torch.full((3 * 2048,), 0x30, **u8), torch.full((5 * 2048,), 0x30,
+                                                           **u8)
+x = torch.randn(400, 2048, device="cuda").half()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c = dg.linear(a, b, sfa, sfb, flags=_lib.LINEAR_PAIR)
+    z = dg.block_norm(x, x)[1]
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(c, dg.linear(a, b, sfa, sfb, flags=_lib.LINEAR_PAIR))
+assert torch.equal(z, dg.block_norm(x, x)[1])
+print("same")
+"""
+
+
+def test_first_pair_and_ring_calls_of_a_process_inside_a_capture():
+    out = subprocess.run([sys.executable, "-c", FIRST_PAIR_IN_CAPTURE],
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("rows,d,gates", [(301, 8256, 7), (700, 16384, 0),
+                                          (310, 20032, 310), (300, 32768, 1)])
+def test_many_rows_wider_than_8192(rows, d, gates, kind, dtype):
+    t = problem(rows, d, dtype, rows, gates, layer_bias=kind == "layer")
+    r, z = dg.block_norm(**t, kind=kind, scale=0.25)
+    want, err = reference(t, r, kind, 0.25)
+    check(z, want, err, "Z")
+    r2, codes, sf = dg.block_norm_nvfp4(**t, kind=kind, scale=0.25)
+    quant = dg.quantize_nvfp4(z, plain=False)
+    assert torch.equal(r, r2)
+    assert torch.equal(codes, quant[0]) and torch.equal(sf, quant[2])
+
+
+def test_mixed_operators_on_two_streams():
+    """Norms with a ring, few-token and pair products of two streams at once
+    give the bits that each gives alone."""
+    m, d, n = 400, 2048, 1032
+    x, y = (torch.randn(m, d, device="cuda").bfloat16() for _ in range(2))
+    b, sfb = linear_operands(1, n, d)[1::2]
+    w = torch.ones(d, device="cuda")
+
+    def step(rows):
+        r, a, sfa = dg.block_norm_nvfp4(x[:rows], y[:rows], weight=w,
+                                        post_weight=w)
+        return r, a, sfa, dg.linear(a, b, sfa, sfb, dtype=x.dtype)
+    sizes = (1, 40, 400)
+    want = {rows: step(rows) for rows in sizes}
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        rows = sizes[i % 3]
+        with torch.cuda.stream(streams[i * 7 // 3 % 2]):
+            got.append((rows, step(rows)))
+    torch.cuda.synchronize()
+    for rows, out in got:
+        for a, e in zip(out, want[rows]):
+            assert torch.equal(a, e)
