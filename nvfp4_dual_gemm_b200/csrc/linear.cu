@@ -320,28 +320,27 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// x / (1 + 2^t) of a pair, given t - kFar: two special-function operations and
-// three packed ones.  The denominator is taken 2^-kFar times as large, and its
-// reciprocal brought back by an exact factor: a reciprocal below 2^-126 is
-// flushed to zero, which would lose results from t = 126 on (silu of x < -87.3)
-// although they are normal numbers of bf16 down to t = 132 and of any
-// consequence to it down to t = 141, the new limit.  Beyond, and where the
-// denominator is infinite, the quotient is a zero.  kFar <= 15 keeps t - kFar
-// below 16 where t is small, so that its rounding costs at most 2^-21.
-// (The reciprocal by Newton steps on the FMA pipe halves the special-function
-// operations and doubles the instructions; the epilogue's few warps wait on
-// instructions, not on that pipe: 16 experts of 1500 rows with silu took 29.7
-// us without them, 31.9 with.)
+// x / (1 + 2^t), given t - kFar: two special-function operations and three
+// others.  The denominator is taken 2^-kFar times as large, and its reciprocal
+// brought back by an exact factor: a reciprocal below 2^-126 is flushed to
+// zero, which would lose results from t = 126 on (silu of x < -87.3) although
+// they are normal numbers of bf16 up to t = 132 and of any consequence to it
+// up to t = 141, the new limit.  Beyond, and where the denominator is infinite,
+// the quotient is a zero.  kFar = 15 keeps t - kFar below 16 where t is small,
+// so that its rounding costs at most 2^-21.
+// (Packed pairs save two instructions of eleven, but the few-token kernels then
+// hold their rows in aligned registers whatever the activation: 1 x 4096 x 4096
+// took 5.90 instead of 5.75 us, 64 experts of 2 rows 16.4 instead of 15.8, 16
+// of ~94 rows with silu the same 27.4.  The reciprocal by Newton steps on the
+// FMA pipe halves the special-function operations and doubles the instructions:
+// the last of these cases took 29.7 us without them, 31.9 with.)
 constexpr float kFar = 15.f;
-__device__ __forceinline__ F2 quotient(F2 x, F2 t) {
+__device__ __forceinline__ float quotient(float x, float t) {
   constexpr float kScale = 1.f / 32768.f;  // 2^-kFar
-  F2 e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-  e = add2(e, {kScale, kScale});
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
-  return mul2(x, mul2(r, {kScale, kScale}));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(kScale + e));
+  return x * (r * kScale);
 }
 
 // Not inlined: 32 copies of erfc would cost the epilogue its registers.
@@ -355,7 +354,6 @@ __device__ __noinline__ float gelu_erf(float x) {
 // 0.5 x erfc(-x / sqrt 2), which keeps its digits for negative x.
 template <int NC>
 __device__ __forceinline__ void activate(float (&v)[NC], int act) {
-  static_assert(NC % 2 == 0, "values go in pairs");
   if (act == NVFP4DG_ACT_NONE) return;
   if (act == NVFP4DG_ACT_RELU) {
 #pragma unroll
@@ -363,22 +361,13 @@ __device__ __forceinline__ void activate(float (&v)[NC], int act) {
   } else if (act == NVFP4DG_ACT_SILU) {
     constexpr float k = -1.4426950408889634f;  // -log2(e)
 #pragma unroll
-    for (int i = 0; i < NC; i += 2) {
-      const F2 x = {v[i], v[i + 1]};
-      const F2 y = quotient(x, fma2({k, k}, x, {-kFar, -kFar}));
-      v[i] = y.x;
-      v[i + 1] = y.y;
-    }
+    for (int i = 0; i < NC; ++i) v[i] = quotient(v[i], fmaf(k, v[i], -kFar));
   } else if (act == NVFP4DG_ACT_GELU_TANH) {
     constexpr float k = -2.302208198201456f;  // -2 sqrt(2/pi) log2(e)
-    constexpr float k3 = 0.044715f * k;
 #pragma unroll
-    for (int i = 0; i < NC; i += 2) {
-      const F2 x = {v[i], v[i + 1]};
-      const F2 u = fma2({k3, k3}, mul2(x, x), {k, k});
-      const F2 y = quotient(x, fma2(x, u, {-kFar, -kFar}));
-      v[i] = y.x;
-      v[i + 1] = y.y;
+    for (int i = 0; i < NC; ++i) {
+      const float x = v[i];
+      v[i] = quotient(x, fmaf(x, fmaf(0.044715f * k, x * x, k), -kFar));
     }
   } else {
 #pragma unroll
