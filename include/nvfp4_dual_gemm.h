@@ -332,11 +332,11 @@ NVFP4DG_API int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream);
 /*
  * The same for `groups` (1..256) products that share N and K but have their
  * own rows, weights and bias: the experts of a mixture, in one launch.  Group
- * g owns rows [row0, row0 + group_rows[g]) of A, SFA, C, residual and
- * row_scale (M rows in all), and batch g of B, SFB (per-batch sizes as for
- * one product) and bias.  First rows are multiples of 128: group_row0, or,
- * when it is NULL, each group starts at the next multiple of 128 after the
- * one before.  Groups may be empty; rows of no group are not written.
+ * g owns rows [row0, row0 + group_rows[g]) of A, SFA, C and row_scale (M rows
+ * in all), and batch g of B, SFB (per-batch sizes as for one product) and
+ * bias; residual must be NULL.  First rows are multiples of 128: group_row0,
+ * or, when it is NULL, each group starts at the next multiple of 128 after
+ * the one before.  Groups may be empty; rows of no group are not written.
  *   on_device == 0: group_rows and group_row0 are host arrays, read during
  *     the call; first rows ascend, and wrong or overlapping groups are
  *     refused (whatever M and N are).
@@ -344,7 +344,11 @@ NVFP4DG_API int nvfp4_linear_run(const nvfp4_linear_args* args, void* stream);
  *     counts without a copy to the host; a captured call reads them at each
  *     replay).  A negative count is an empty group; a group whose first row
  *     lies outside A or is no multiple of 128 is empty, and one that reaches
- *     past row M is cut there.  Groups must not overlap.
+ *     past row M is cut there.  Groups must not overlap.  The host, which
+ *     does not see the counts, chooses the tile by M: for an A with room for
+ *     many more rows than its groups have (a captured decode step with space
+ *     for the largest one), force a small one with NVFP4DG_LINEAR_TOKENS32
+ *     or _TOKENS64.
  */
 NVFP4DG_API int nvfp4_linear_run_grouped(const nvfp4_linear_args* args,
                                          const int* group_rows,
@@ -368,7 +372,8 @@ NVFP4DG_API int nvfp4_linear_plan(int M, int N, int K, int residual,
  *   z = norm(r) * weight + bias               (of the rounded r)
  *
  * norm is v / sqrt(mean(v^2) + eps) (NVFP4DG_NORM_RMS) or
- * (v - mean(v)) / sqrt(var(v) + eps) (NVFP4DG_NORM_LAYER), in fp32.  A NULL
+ * (v - mean(v)) / sqrt(var(v) + eps) (NVFP4DG_NORM_LAYER), in fp32, squares
+ * too: a row whose squares sum to more than 3.4e38 gives zeros.  A NULL
  * weight is 1, a NULL bias 0, a NULL gate 1.  With y == NULL, r is x and R is
  * not written.  gate is [gate_rows, D] of the stream's type, row i of it for
  * the i-th of gate_rows equal runs of rows (1: one gate for all; rows: one

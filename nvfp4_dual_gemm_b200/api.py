@@ -344,7 +344,12 @@ def linear_grouped(A, B, SFA, SFB, C, group_rows, group_row0=None, *,
     their rows.  Up to 256 groups, any of them empty; rows of no
     group are not written.  Counts on the host are checked; on the device, a
     group that is out of place is empty and one that reaches past the rows of
-    A or C is cut there (``nvfp4_linear_run_grouped``)."""
+    A or C is cut there (``nvfp4_linear_run_grouped``).
+
+    With counts on the device the tile is chosen by the rows of A and C, since
+    the host does not see the counts.  Where they have room for many more rows
+    than the groups (a captured decode step with space for the largest one),
+    force a small tile: ``flags=_lib.LINEAR_TOKENS32`` or ``_TOKENS64``."""
     return _lib.ext().linear_grouped(A, B, SFA, SFB, C, group_rows,
                                      group_row0, bias, activation, row_scale,
                                      alpha, flags)

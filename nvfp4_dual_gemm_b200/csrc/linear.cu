@@ -1146,22 +1146,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 // token row; outputs leave through shared memory and TMA stores, 64 columns
 // at a time.
 //
-// Bound by the ring's latency: a stage's tiles land ~2100 cycles after it is
-// free, its MMAs take 512 and the hand-offs ~1000, so that five stages give a
-// block every ~740 cycles where the tensor cores need 512; then by power
-// (timed in turns with short pauses: 8192 x 8192 x 28672 768 us, 5.0 PFLOP/s;
-// 4096 x 4096 x 14336 with a residual 115 us, 4.2 PFLOP/s).  There is one
-// accumulator, and a tile's epilogue takes ~6000 cycles: so its 256 columns go
-// to registers at once and the next tile's products start under it (126 ->
-// 115 us and 781 -> 768 us for the two, 122 -> 114 us for 32 experts of 512
-// rows and K 2048; a tile whose rows are stored one by one is slower, 37 ->
-// 39 us for 16 experts of ~94 rows, which the schedule gives smaller tiles).
-// That needs 192 registers in the epilogue's threads and hence the warpgroups'
-// shares; a spilled register costs more than elsewhere, as shared memory
-// leaves next to no L1.  Tried and slower: sixteen epilogue warps with half the
-// columns each, outputs stored without boxes, the columns in four rounds
-// through 64 registers (122 -> 139 us), and scales copied ahead of their stage
-// (two waits in the scale warps: no gain).
+// Up to K of ~2500 bound by a tile's epilogue, 9,000 cycles at K 512 and
+// 10,300 at K 2048 by stamps in steady state: ~1,400 from a tile's last store
+// until the next accumulator is seen full (the tile's place, its bias, the
+// wait), ~450 for the columns to registers, the rest for four chunks of 32
+// columns; the products of the next tile start ~1,200 cycles after the
+// accumulator was full and are done before its epilogue begins.  A residual,
+// read by 16-byte loads of 32 rows a warp, adds ~6,000 to the chunks.  592
+// tiles, 8 a pair, take 42.6 us for K of 64, 44.8 for 512, 53.4 for 2048; with
+// a residual 71, 72 and 82.
+// For longer K bound by a K block's ~740 cycles, where its MMAs take 512, and
+// ~2,400 a tile between its last product and the next one's first (118 us for
+// K of 7168).  Not by the ring's latency: 72 tiles, one a pair, take 424 ns a
+// block with five stages, 445 with four, 550 with three, where latency alone
+// would give 530 and 707.  Not by the copies either, if the dual GEMM's pair
+// loop is a guide, whose block of the same size takes as long with its tile
+// copies left out.  The cause is open.
+// In a long loop by power.  (In turns with short pauses: 8192 x 8192 x 28672
+// 746 us, 5.2 PFLOP/s; 4096 x 4096 x 14336 with a residual 112 us, 4.3.)
+// There is one accumulator: its 256 columns go to registers at once and the
+// next tile's products start under the epilogue (126 -> 115 us and 781 -> 768
+// us for the two when that was brought in, 122 -> 114 us for 32 experts of
+// 16384 rows and K 2048; a tile whose rows are stored one by one is slower, 37
+// -> 39 us for 16 experts of ~94 rows, which the schedule gives smaller
+// tiles).  That needs 192 registers in the epilogue's threads and hence the
+// warpgroups' shares; a spilled register costs more than elsewhere, as shared
+// memory leaves next to no L1.  Tried and slower: sixteen epilogue warps with
+// half the columns each, outputs stored without boxes, the columns in four
+// rounds through 64 registers (122 -> 139 us), and scales copied ahead of
+// their stage (two waits in the scale warps: no gain).
 // ---------------------------------------------------------------------------
 constexpr int kPairThreads = 512;
 // Whole warpgroups, whose shares of the launch's registers follow their work:
@@ -1666,11 +1679,12 @@ struct LinearPlan {
 };
 
 // What a launch takes, in microseconds, fitted to B200 timings of 1 to 4000
-// tokens (N 512 to 8192, K 512 to 14336, graph-replayed, L2 warm): a start and
-// end, the first wave of tiles, and every further one, which is bound by its
-// products or by its epilogue.  `kb`: the 256-wide K blocks of a CTA;
-// `tokens`: 0 for groups, whose tiles say it all.  (500 x 8192 x 512: 8.2 us
-// with 128 tokens, 10.2 with pairs; x 7168: 27.0 and 20.1.)
+// tokens (N 512 to 8192, K 512 to 14336, graph-replayed, L2 warm, single
+// problems): a start and end, the first wave of tiles, and every further one,
+// which is bound by its products or by its epilogue.  `kb`: the 256-wide K
+// blocks of a CTA; `tokens`: 0 for groups, whose tiles say it all and which the
+// constants were not fitted to.  (500 x 8192 x 512: 8.2 us with 128 tokens,
+// 10.2 with pairs; x 7168: 27.0 and 20.1.)
 double linear_cost(int tn, double kb, double waves, bool split, int tokens,
                    bool residual) {
   if (tn == 32) {
@@ -1997,8 +2011,12 @@ int run_linear(const nvfp4_linear_args* a, const int* group_rows,
     tokens = mt[0] * 32;
   } else {
     if (a->M == 0 || a->N == 0) return NVFP4DG_OK;
-    // counts on the device: A's rows spread evenly, most of a row block of
-    // each group taken for padding
+    // counts on the device: A's rows spread evenly.  A tight A pads each
+    // group to 128 rows, by 127 at most and 64 on average; 96 are taken off,
+    // but no more than three quarters.  An A sized for more rows than there
+    // are gets the tile of those (32 experts of 4 rows, each in 256 rows of A,
+    // 4096 x 2048: 44 us with the pairs this gives, 28 with 32 tokens), which
+    // a tile flag prevents.
     long long per = groups ? (a->M + groups - 1) / groups : a->M;
     if (groups) per = std::max(per - 96, (per + 3) / 4);
     tokens = per * std::max(groups, 1);

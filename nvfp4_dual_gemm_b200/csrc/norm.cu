@@ -11,7 +11,8 @@
 // rows wider than a warp holds, one word a warp in shared memory.
 //
 // Bound by memory for many wide rows (8192 x 7168 bf16, post and pre RMS norm:
-// 75 us, 6.3 TB/s, 0.96 of the measured copy bandwidth), by instructions for
+// 75 us replayed from a graph, 6.3 TB/s, 0.96 of the measured copy bandwidth;
+// 82 us a call in a long loop), by instructions for
 // narrower ones (10800 x 2056: 38 us, 4.7 TB/s; layer norms 52 us), by latency
 // for few (1 x 7168: 3.0 us).
 #include <cuda_bf16.h>
